@@ -41,12 +41,17 @@ extern "C" {
 #define SK_API
 #endif
 
-#define SK_ABI_VERSION 8
+#define SK_ABI_VERSION 9
 
 /* Element type codes. */
 #define SK_F32 0
 #define SK_F16 1
 #define SK_BF16 2
+
+/* Code types of an 8-bit cache (sk_kv_cache_update_q8, sk_attn_q8): int8, and
+ * float8 e4m3 in the OCP encoding (largest finite value 448, no infinities). */
+#define SK_I8 3
+#define SK_E4M3 4
 
 /* Error codes (negative: argument rejected before any launch). */
 #define SK_OK 0
@@ -495,6 +500,111 @@ SK_API int sk_kv_cache_update_paged_rope(int dtype, const void* k, const void* v
 SK_API int sk_kernel_config(int op, int dtype, int B, int Hq, int Hkv, int Sq, int Sk, int D,
                      int is_causal, int num_splits, int variant, int query_device,
                      int64_t* cfg, char* kernel_name, size_t name_len);
+
+/* ------------------------------------------------------------ 8-bit cache */
+
+/*
+ * Page plan of a serving step: block tables and slot maps from request lengths,
+ * on the device.  Row b holds lens[b] = clamp(cache_seqlens[b], 0, max_pages *
+ * page_size) tokens in the pages block_table[b, 0 .. ceil(lens[b] / page_size)).
+ * new_lens[b] > 0: it grows by min(new_lens[b], max_new) tokens; < 0: its last
+ * -new_lens[b] tokens go (all, where it holds fewer).
+ *
+ * free_pages is a ring of num_free page ids, free_state = {head, count} the
+ * place of its first id and how many there are.  Rows that grow take pages from
+ * the front in row order and store them in block_table behind those they hold; a
+ * row that does not fit its table, or whose pages (summed over it and the rows
+ * before it that fit theirs) exceed count, does not grow at all.  Rows that
+ * shrink put the pages they no longer need behind the ring's end in row order
+ * (usable from the next call on; their table entries stay as they are; ids that
+ * would not fit the ring are dropped).
+ *
+ * Writes slots (B, max_new): page * page_size + in-page row of each new token,
+ * -1 past a row's new tokens, for one that was refused and in a page < 0;
+ * seqlens_out (B), the new lengths; state_out {head, count}.  seqlens_out and
+ * state_out must not overlap the inputs.  The call reads no entry that it writes,
+ * so the same inputs give the same outputs again.  B * max_pages < 2^31.
+ */
+SK_API int sk_kv_page_plan(int32_t* block_table, const int32_t* cache_seqlens,
+                    const int32_t* new_lens, int32_t* free_pages, const int32_t* free_state,
+                    int64_t* slots, int32_t* seqlens_out, int32_t* state_out, int B,
+                    int max_pages, int64_t table_stride, int page_size, int max_new,
+                    int num_free, void* stream);
+
+/*
+ * Append to a cache of 8-bit codes with one fp32 scale per block of block_size
+ * tokens and KV head (an element's value is scale * code).  Token t < new_lens[b]
+ * (NULL: T; clamped to [0, T]) of batch row b of k, v (B, Hkv, T, D) becomes
+ * token max(cache_seqlens[b], 0) + t of row b.
+ *
+ * units = B, rows = S_cache, block_table NULL: the caches are (B, Hkv, S_cache,
+ * D), their scales (B, Hkv, ceil(S_cache / block_size)).  Else they are pools of
+ * units pages of rows = page_size tokens with scales (units, Hkv, page_size /
+ * block_size), token n of row b in page block_table[b, n / page_size] of (B,
+ * max_pages).  Tokens past the row's capacity or in a page outside the pool are
+ * skipped; two batch rows must not write the same block.
+ *
+ * A block takes the scale its new values need (int8: largest magnitude / 127;
+ * e4m3: the smallest power of two that brings it to 448 or less; at least 2^-126;
+ * infinities and NaN do not count), or keeps its own where it holds older tokens
+ * of the row and its own is larger; where it grows, the older tokens' codes are
+ * rounded to the new scale.  New codes are round(x * (1 / scale)), ties to even,
+ * saturated; NaN becomes 0 in int8 and NaN in e4m3.  Rows of the cache behind a
+ * row's last token are left as they are.
+ *
+ * With tables (rope_cos non-NULL) the new keys are rotated first, token t at
+ * position rope_pos[b] + rope_start + t, in fp32 and not rounded in between.
+ *
+ * D: a multiple of 16 up to 256.  block_size: a multiple of 32 that divides
+ * page_size.  Pointers to k, v and codes are 16-byte aligned, k, v strides
+ * multiples of 8 elements (4 for fp32), code strides multiples of 16; scale
+ * strides are int64_t[3] = {unit, head, block}.
+ */
+SK_API int sk_kv_cache_update_q8(int dtype, int code, const void* k, const void* v, void* k_cache,
+                          void* v_cache, float* k_scale, float* v_scale,
+                          const int32_t* cache_seqlens, const int32_t* new_lens,
+                          const int32_t* block_table, int B, int Hkv, int T, int units, int rows,
+                          int max_pages, int block_size, int D, const int64_t* k_strides,
+                          const int64_t* v_strides, const int64_t* kc_strides,
+                          const int64_t* vc_strides, const int64_t* ks_strides,
+                          const int64_t* vs_strides, const void* rope_cos, const void* rope_sin,
+                          int rope_dtype, int rope_rows, int64_t rope_stride,
+                          const int32_t* rope_pos, int rope_start, void* stream);
+
+/*
+ * Split count and scratch bytes that sk_attn_q8 takes for a shape (Sk: the most
+ * keys a row can have, S_cache or max_pages * page_size).
+ */
+SK_API int sk_attn_q8_plan(int dtype, int B, int Hq, int Hkv, int Sq, int Sk, int D, int is_causal,
+                    int* num_splits, size_t* workspace_bytes);
+
+/*
+ * Attention of Sq >= 1 query tokens per batch row over a cache of 8-bit codes
+ * (the format of sk_kv_cache_update_q8; scales may be any fp32 numbers).
+ *
+ *   q (B, Hq, Sq, D) -> o (B, Hq, Sq, D) of q's dtype.
+ *
+ * Row b has len = clamp(cache_seqlens[b], 0, Sk) keys (NULL: Sk, contiguous
+ * caches only) and n = clamp(query_lens[b], 0, Sq) queries (NULL: Sq); with
+ * is_causal query i < n sees the keys j <= len - n + i, else all len.  Queries i
+ * >= n, and those that see no key, give zeros.  Keys in a page outside the pool
+ * are left out.  Nothing past a row's length is read.  Queries are rotated as in
+ * sk_attn_fwd_rope when rope_cos is given: query i at rope_pos[b] + rope_start + i.
+ *
+ * num_splits 0 takes the plan's count; workspace must hold (D padded to 64, 128 or
+ * 256, + 1) * 4 * B * Hq * Sq bytes per split when it is above 1.  Limits on D,
+ * block_size, alignment and strides as above; a code row stride is 0 or at least D.
+ */
+SK_API int sk_attn_q8(int dtype, int code, const void* q, const void* k_cache, const void* v_cache,
+               const float* k_scale, const float* v_scale, void* o, void* workspace,
+               size_t workspace_bytes, int num_splits, int B, int Hq, int Hkv, int Sq, int units,
+               int rows, int max_pages, int block_size, int D, const int64_t* q_strides,
+               const int64_t* kc_strides, const int64_t* vc_strides, const int64_t* ks_strides,
+               const int64_t* vs_strides, const int64_t* o_strides, const int32_t* block_table,
+               const int32_t* cache_seqlens, const int32_t* query_lens, int is_causal,
+               const void* rope_cos, const void* rope_sin, int rope_dtype, int rope_rows,
+               int64_t rope_stride, const int32_t* rope_pos, int rope_start, float sm_scale,
+               void* stream);
 
 #ifdef __cplusplus
 }

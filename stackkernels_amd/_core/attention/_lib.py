@@ -15,8 +15,9 @@ import os
 import threading
 
 SK_F32, SK_F16, SK_BF16 = 0, 1, 2
+SK_I8, SK_E4M3 = 3, 4
 SK_OK, SK_EINVAL, SK_EUNSUPPORTED, SK_EWORKSPACE = 0, -1, -2, -3
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 _LIB_DIR = os.path.join(os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__)))), "csrc")
 LIB_PATH = os.environ.get("SK_ATTN_LIB", os.path.join(_LIB_DIR, "libsk_attn.so"))
@@ -34,6 +35,7 @@ _intp = ctypes.POINTER(ctypes.c_int)
 # name -> (restype, argtypes); mirrors include/sk_attn.h.
 # RoPE arguments: cos, sin, table dtype, rows, row stride, positions, start.
 _ROPE = (_vp, _vp, _c_int, _c_int, ctypes.c_int64, _vp, _c_int)
+NO_ROPE = (None, None, 0, 0, 0, None, 0)  # where a call's rotation is optional
 
 SIGNATURES: dict[str, tuple] = {
     "sk_abi_version": (_c_int, []),
@@ -98,6 +100,18 @@ SIGNATURES: dict[str, tuple] = {
     "sk_kv_cache_update_paged_rope": (_c_int, [_c_int, _vp, _vp, _vp, _vp, _vp,
                                                _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                                _i64p, _i64p, _i64p, _i64p, *_ROPE, _vp]),
+    "sk_kv_page_plan": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int,
+                                 ctypes.c_int64, _c_int, _c_int, _c_int, _vp]),
+    "sk_kv_cache_update_q8": (_c_int, [_c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                       _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                       _c_int, _i64p, _i64p, _i64p, _i64p, _i64p, _i64p, *_ROPE,
+                                       _vp]),
+    "sk_attn_q8_plan": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                 _intp, _sizep]),
+    "sk_attn_q8": (_c_int, [_c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t,
+                            _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                            _c_int, _c_int, _i64p, _i64p, _i64p, _i64p, _i64p, _i64p, _vp, _vp,
+                            _vp, _c_int, *_ROPE, _c_float, _vp]),
     "sk_kernel_config": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                   _c_int, _c_int, _c_int, _c_int, _i64p, ctypes.c_char_p,
                                   ctypes.c_size_t]),
@@ -167,6 +181,18 @@ def dtype_code(dtype) -> int:
     if dtype == torch.float32:
         return SK_F32
     raise NotImplementedError(f"dtype {dtype} has no HIP kernel (supported: float32, float16, bfloat16)")
+
+
+def code_type(dtype) -> int:
+    """Code of an 8-bit cache's element type."""
+    import torch
+
+    if dtype == torch.int8:
+        return SK_I8
+    if dtype == torch.float8_e4m3fn:
+        return SK_E4M3
+    raise NotImplementedError(f"cache dtype {dtype} has no HIP kernel (supported: int8, "
+                              "float8_e4m3fn)")
 
 
 def stream_ptr(device) -> int:

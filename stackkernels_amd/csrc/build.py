@@ -20,7 +20,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(os.path.dirname(HERE))
 INCLUDE = os.path.join(REPO, "include")
 SOURCES = ["sk_abi.hip", "sk_fwd.hip", "sk_decode.hip", "sk_fp32.hip", "sk_bwd.hip", "sk_cache.hip",
-           "sk_rotate.hip"]
+           "sk_rotate.hip", "sk_cache_q8.hip", "sk_attn_q8.hip"]
 LIB_NAME = "libsk_attn.so"
 ARCH = "gfx950"
 

@@ -12,6 +12,7 @@
 
 #include "sk_attn.h"
 #include "sk_kernels.h"
+#include "sk_q8.h"
 
 namespace {
 
@@ -1038,6 +1039,249 @@ int sk_rope_rotate(int dtype, const void* x, void* out, int B, int H, int S, int
   p.rope = r;
   const hipError_t e = sk::launch_rope_rotate(p, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "sk_rope_rotate launch");
+  return SK_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- 8-bit cache
+
+// The format's shape rules shared by the append and the attention.
+static int check_q8(int dtype, int code, int B, int Hkv, int units, int rows, int max_pages,
+                    bool paged, int block_size, int D) {
+  if (dtype != SK_F32 && dtype != SK_F16 && dtype != SK_BF16)
+    return fail(SK_EUNSUPPORTED, "unsupported dtype code %d", dtype);
+  if (code != SK_I8 && code != SK_E4M3)
+    return fail(SK_EUNSUPPORTED, "unsupported code type %d (int8 or float8 e4m3)", code);
+  if (B < 0 || Hkv <= 0 || units < 0 || rows < 0 || max_pages < 0 || D <= 0)
+    return fail(SK_EINVAL, "invalid sizes B=%d Hkv=%d units=%d rows=%d max_pages=%d D=%d", B, Hkv,
+                units, rows, max_pages, D);
+  if (D % 16 != 0 || D > 256)
+    return fail(SK_EUNSUPPORTED, "head dim %d unsupported: need a multiple of 16 up to 256", D);
+  if (block_size <= 0 || block_size % 32 != 0)
+    return fail(SK_EINVAL, "block_size=%d must be a positive multiple of 32", block_size);
+  if (paged) {
+    if (rows <= 0 || rows % block_size != 0)
+      return fail(SK_EINVAL, "page_size=%d must be a positive multiple of block_size=%d", rows,
+                  block_size);
+    if (max_pages > 0 && units == 0) return fail(SK_EINVAL, "empty page pool");
+    if ((int64_t)max_pages * rows > 0x7fff0000LL)
+      return fail(SK_EINVAL, "max_pages * page_size overflows int");
+  } else if (units != B) {
+    return fail(SK_EINVAL, "a contiguous cache of %d rows for a batch of %d", units, B);
+  } else if (rows > 0x7fff0000) {
+    return fail(SK_EINVAL, "cache of %d tokens is too long", rows);
+  }
+  return SK_OK;
+}
+
+// Code and scale strides -> c.  Rows of codes may not overlap in part (a load of
+// a row's last bytes would then read rows behind the visible ones).
+static int make_q8_cache(const char* name, const void* codes, const float* scales,
+                         const int64_t* st, const int64_t* sst, int D, sk::Q8Cache* c) {
+  if (!st || !sst) return fail(SK_EINVAL, "%s strides pointer is NULL", name);
+  for (int i = 0; i < 3; ++i) {
+    if (st[i] < 0 || st[i] % 16 != 0)
+      return fail(SK_EINVAL, "%s stride[%d]=%lld must be a non-negative multiple of 16 elements",
+                  name, i, (long long)st[i]);
+    if (sst[i] < 0)
+      return fail(SK_EINVAL, "%s scale stride[%d]=%lld must be non-negative", name, i,
+                  (long long)sst[i]);
+  }
+  if (st[2] != 0 && st[2] < D)
+    return fail(SK_EINVAL, "%s row stride %lld is less than the head dim %d", name,
+                (long long)st[2], D);
+  if (st[2] > (1LL << 25))
+    return fail(SK_EINVAL, "%s row stride %lld is too large", name, (long long)st[2]);
+  c->codes = (uint8_t*)const_cast<void*>(codes);
+  c->scales = const_cast<float*>(scales);
+  c->sb = st[0], c->sh = st[1], c->ss = st[2];
+  c->cb = sst[0], c->ch = sst[1], c->cs = sst[2];
+  return SK_OK;
+}
+
+// Whether [a, a + an) and [b, b + bn) share a byte.
+static bool overlap(const void* a, size_t an, const void* b, size_t bn) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return x < y + bn && y < x + an;
+}
+
+static size_t q8_ws_bytes(int B, int Hq, int Sq, int D, int splits) {
+  return splits <= 1 ? 0 : (size_t)B * Hq * Sq * splits * (sk::q8_dpad(D) + 1) * sizeof(float);
+}
+
+extern "C" {
+
+int sk_kv_page_plan(int32_t* block_table, const int32_t* cache_seqlens, const int32_t* new_lens,
+                    int32_t* free_pages, const int32_t* free_state, int64_t* slots,
+                    int32_t* seqlens_out, int32_t* state_out, int B, int max_pages,
+                    int64_t table_stride, int page_size, int max_new, int num_free, void* stream) {
+  g_err[0] = 0;
+  if (B < 0 || max_pages < 0 || max_new < 0)
+    return fail(SK_EINVAL, "invalid sizes B=%d max_pages=%d max_new=%d", B, max_pages, max_new);
+  if (page_size <= 0) return fail(SK_EINVAL, "page_size=%d must be positive", page_size);
+  if (num_free <= 0) return fail(SK_EINVAL, "free_pages must hold at least one id");
+  if (table_stride < max_pages)
+    return fail(SK_EINVAL, "block_table row stride %lld is less than max_pages=%d",
+                (long long)table_stride, max_pages);
+  if ((int64_t)max_pages * page_size > 0x7fff0000LL)
+    return fail(SK_EINVAL, "max_pages * page_size overflows int");
+  if ((int64_t)B * max_pages > 0x7fffffffLL) return fail(SK_EINVAL, "B * max_pages overflows int");
+  if (B == 0) return SK_OK;
+  const void* ptrs[7] = {cache_seqlens, new_lens, free_pages, free_state, seqlens_out, state_out,
+                         max_pages > 0 ? (const void*)block_table : (const void*)free_pages};
+  const char* names[7] = {"cache_seqlens", "new_lens", "free_pages", "free_state", "seqlens_out",
+                          "state_out", "block_table"};
+  for (int i = 0; i < 7; ++i)
+    if (!ptrs[i]) return fail(SK_EINVAL, "%s pointer is NULL", names[i]);
+  if (max_new > 0 && !slots) return fail(SK_EINVAL, "slots pointer is NULL");
+  if (overlap(seqlens_out, 4 * (size_t)B, cache_seqlens, 4 * (size_t)B) ||
+      overlap(seqlens_out, 4 * (size_t)B, new_lens, 4 * (size_t)B) ||
+      overlap(state_out, 8, free_state, 8))
+    return fail(SK_EINVAL, "seqlens_out and state_out must not overlap the inputs");
+  sk::PagePlanParams p{};
+  p.table = block_table, p.table_stride = table_stride;
+  p.lens = cache_seqlens, p.news = new_lens;
+  p.ring = free_pages, p.state = free_state;
+  p.slots = slots, p.lens_out = seqlens_out, p.state_out = state_out;
+  p.B = B, p.max_pages = max_pages, p.page_size = page_size, p.T = max_new, p.N = num_free;
+  const hipError_t e = sk::launch_page_plan(p, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "sk_kv_page_plan launch");
+  return SK_OK;
+}
+
+int sk_kv_cache_update_q8(int dtype, int code, const void* k, const void* v, void* k_cache,
+                          void* v_cache, float* k_scale, float* v_scale,
+                          const int32_t* cache_seqlens, const int32_t* new_lens,
+                          const int32_t* block_table, int B, int Hkv, int T, int units, int rows,
+                          int max_pages, int block_size, int D, const int64_t* k_strides,
+                          const int64_t* v_strides, const int64_t* kc_strides,
+                          const int64_t* vc_strides, const int64_t* ks_strides,
+                          const int64_t* vs_strides, const void* rope_cos, const void* rope_sin,
+                          int rope_dtype, int rope_rows, int64_t rope_stride,
+                          const int32_t* rope_pos, int rope_start, void* stream) {
+  g_err[0] = 0;
+  const bool paged = block_table != nullptr || max_pages > 0;
+  int rc = check_q8(dtype, code, B, Hkv, units, rows, max_pages, paged, block_size, D);
+  if (rc) return rc;
+  if (T < 0) return fail(SK_EINVAL, "invalid T=%d", T);
+  sk::Q8AppendParams p{};
+  if ((rc = check_strides(dtype, "k", k_strides)) || (rc = check_strides(dtype, "v", v_strides)) ||
+      (rc = make_q8_cache("k_cache", k_cache, k_scale, kc_strides, ks_strides, D, &p.c[0])) ||
+      (rc = make_q8_cache("v_cache", v_cache, v_scale, vc_strides, vs_strides, D, &p.c[1])))
+    return rc;
+  for (int i = 0; i < 2; ++i)
+    if (rows > 1 && p.c[i].ss == 0) return fail(SK_EINVAL, "cache rows overlap (row stride 0)");
+  if (rope_cos || rope_sin) {
+    if ((rc = make_rope(rope_cos, rope_sin, rope_dtype, rope_rows, rope_stride, rope_pos,
+                        rope_start, D, B > 0 ? T : 0, &p.rope)))
+      return rc;
+  }
+  if ((int64_t)B * T == 0 || rows == 0 || (paged && max_pages == 0)) return SK_OK;
+  if (paged && !block_table) return fail(SK_EINVAL, "block_table pointer is NULL");
+  if ((rc = check_ptr("k", k)) || (rc = check_ptr("v", v)) || (rc = check_ptr("k_cache", k_cache)) ||
+      (rc = check_ptr("v_cache", v_cache)))
+    return rc;
+  if (!k_scale || !v_scale || !cache_seqlens)
+    return fail(SK_EINVAL, "%s pointer is NULL",
+                !k_scale ? "k_scale" : !v_scale ? "v_scale" : "cache_seqlens");
+  p.x[0] = k, p.x[1] = v;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t* st = i ? v_strides : k_strides;
+    p.x_sb[i] = st[0], p.x_sh[i] = st[1], p.x_ss[i] = st[2];
+  }
+  p.lens = cache_seqlens, p.news = new_lens, p.table = paged ? block_table : nullptr;
+  p.B = B, p.Hkv = Hkv, p.T = T, p.D = D;
+  p.cap = paged ? max_pages * rows : rows;
+  p.page_size = rows, p.max_pages = max_pages, p.num_pages = units;
+  p.block = block_size;
+  p.blocks = (int)(((int64_t)T + block_size - 2) / block_size + 1);
+  if ((int64_t)B * p.blocks * Hkv * 2 * 256 > 0xffffffffLL)
+    return fail(SK_EINVAL, "grid too large: %d rows of %d new tokens, %d heads", B, T, Hkv);
+  const hipError_t e = sk::launch_q8_append(dtype, code, p, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "sk_kv_cache_update_q8 launch");
+  return SK_OK;
+}
+
+int sk_attn_q8_plan(int dtype, int B, int Hq, int Hkv, int Sq, int Sk, int D, int is_causal,
+                    int* num_splits, size_t* workspace_bytes) {
+  g_err[0] = 0;
+  const int rc = check_dims(dtype, B, Hq, Hkv, Sq, Sk, D);
+  if (rc) return rc;
+  if (!num_splits || !workspace_bytes) return fail(SK_EINVAL, "output pointer is NULL");
+  if ((int64_t)Sq * (Hq / Hkv) > 0x7fff0000LL) return fail(SK_EINVAL, "Sq * group overflows int");
+  *num_splits = sk::q8_splits(dtype, B, Hkv, Sq * (Hq / Hkv), Sk, D);
+  *workspace_bytes = q8_ws_bytes(B, Hq, Sq, D, *num_splits);
+  return SK_OK;
+}
+
+int sk_attn_q8(int dtype, int code, const void* q, const void* k_cache, const void* v_cache,
+               const float* k_scale, const float* v_scale, void* o, void* workspace,
+               size_t workspace_bytes, int num_splits, int B, int Hq, int Hkv, int Sq, int units,
+               int rows, int max_pages, int block_size, int D, const int64_t* q_strides,
+               const int64_t* kc_strides, const int64_t* vc_strides, const int64_t* ks_strides,
+               const int64_t* vs_strides, const int64_t* o_strides, const int32_t* block_table,
+               const int32_t* cache_seqlens, const int32_t* query_lens, int is_causal,
+               const void* rope_cos, const void* rope_sin, int rope_dtype, int rope_rows,
+               int64_t rope_stride, const int32_t* rope_pos, int rope_start, float sm_scale,
+               void* stream) {
+  g_err[0] = 0;
+  const bool paged = block_table != nullptr || max_pages > 0;
+  int rc = check_q8(dtype, code, B, Hkv, units, rows, max_pages, paged, block_size, D);
+  if (rc) return rc;
+  const int Sk = paged ? max_pages * rows : rows;
+  if ((rc = check_dims(dtype, B, Hq, Hkv, Sq, Sk, D))) return rc;
+  sk::Q8AttnParams p{};
+  if ((rc = check_strides(dtype, "q", q_strides)) || (rc = check_strides(dtype, "o", o_strides)) ||
+      (rc = make_q8_cache("k_cache", k_cache, k_scale, kc_strides, ks_strides, D, &p.k)) ||
+      (rc = make_q8_cache("v_cache", v_cache, v_scale, vc_strides, vs_strides, D, &p.v)))
+    return rc;
+  if (rope_cos || rope_sin) {
+    if ((rc = make_rope(rope_cos, rope_sin, rope_dtype, rope_rows, rope_stride, rope_pos,
+                        rope_start, D, B > 0 ? Sq : 0, &p.rope)))
+      return rc;
+  }
+  if ((int64_t)B * Hq * Sq == 0) return SK_OK;
+  if ((rc = check_ptr("q", q)) || (rc = check_ptr("o", o))) return rc;
+  if (Sk > 0 && ((rc = check_ptr("k_cache", k_cache)) || (rc = check_ptr("v_cache", v_cache))))
+    return rc;
+  if (Sk > 0 && (!k_scale || !v_scale))
+    return fail(SK_EINVAL, "%s pointer is NULL", !k_scale ? "k_scale" : "v_scale");
+  if (paged && Sk > 0 && (!block_table || !cache_seqlens))
+    return fail(SK_EINVAL, "block_table and cache_seqlens are required");
+  if ((int64_t)Sq * (Hq / Hkv) > 0x7fff0000LL) return fail(SK_EINVAL, "Sq * group overflows int");
+  p.q = q, p.o = o;
+  p.q_sb = q_strides[0], p.q_sh = q_strides[1], p.q_ss = q_strides[2];
+  p.o_sb = o_strides[0], p.o_sh = o_strides[1], p.o_ss = o_strides[2];
+  p.B = B, p.Hq = Hq, p.Hkv = Hkv, p.Sq = Sq, p.Sk = Sk, p.D = D, p.group = Hq / Hkv;
+  p.rows = Sq * p.group;
+  if (num_splits == 0) num_splits = sk::q8_splits(dtype, B, Hkv, p.rows, Sk, D);
+  if (num_splits < 1 || num_splits > 1024)
+    return fail(SK_EINVAL, "num_splits=%d outside [1, 1024]", num_splits);
+  const size_t need = q8_ws_bytes(B, Hq, Sq, D, num_splits);
+  if (need > 0 && (rc = check_ptr("workspace", workspace)))
+    return fail(SK_EWORKSPACE, "workspace pointer is NULL or not 16-byte aligned");
+  if (need > workspace_bytes)
+    return fail(SK_EWORKSPACE, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
+  p.num_splits = num_splits;
+  p.dpad = sk::q8_dpad(D);
+  const int per = sk::q8_rows_per_block(dtype, D, p.rows);
+  p.row_blocks = (p.rows + per - 1) / per;
+  if ((int64_t)B * Hkv * num_splits * p.row_blocks * 256 > 0xffffffffLL ||
+      (num_splits > 1 && (int64_t)B * Hq * Sq * 256 > 0xffffffffLL))
+    return fail(SK_EINVAL, "grid too large: %d rows of %d queries, %d heads, %d splits", B, Sq, Hq,
+                num_splits);
+  if (num_splits > 1) {
+    p.part_o = (float*)workspace;
+    p.part_lse = p.part_o + (size_t)B * Hq * Sq * num_splits * p.dpad;
+  }
+  p.causal = is_causal != 0;
+  p.block = block_size;
+  p.scale_log2 = sm_scale * 1.4426950408889634f;
+  p.seqlens = cache_seqlens, p.qlens = query_lens, p.table = paged ? block_table : nullptr;
+  p.page_size = rows, p.max_pages = max_pages, p.num_pages = units;
+  const hipError_t e = sk::launch_q8_attn(dtype, code, p, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(e, "sk_attn_q8 launch");
   return SK_OK;
 }
 

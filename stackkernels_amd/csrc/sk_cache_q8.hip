@@ -1,0 +1,411 @@
+// Writing a cache held in 8-bit codes, and the page plan of a serving step.
+//
+// Append.  A block of block_size tokens of a KV head has one scale s; the value
+// of a code c is s c.  New values x of a block ask for
+//   int8: amax / 127;  e4m3: the smallest power of two 2^e with amax 2^-e <= 448
+// (amax over the finite ones; at least 2^-126), and the block takes s' = that,
+// or the larger of that and s where the block already holds tokens.  New codes
+// are round(x * (1 / s')), saturated; where s' > s the older codes become
+// round(c * (s / s')).  In e4m3 that factor is a power of two, so older codes
+// keep their value exactly down to the subnormal range: moving a block's scale
+// several times costs no more than moving it once.  In int8 each move rounds
+// once more, by at most half a step of the new scale.
+//
+// One workgroup owns a (batch row, block, KV head, k or v): amax, scale and codes
+// need no atomics and results do not depend on order.  Bound by the new tokens'
+// bytes (2 or 4 in, 1 out per element); the older codes of a block are read only
+// when its scale grows.
+#include <type_traits>
+
+#include "sk_common.h"
+#include "sk_q8.h"
+#include "sk_rope.h"
+
+namespace sk {
+
+constexpr float kTinyScale = 1.17549435e-38f;  // 2^-126
+
+template <int CODE>
+__device__ __forceinline__ float needed_scale(float amax) {
+  if constexpr (CODE == kCodeI8) {
+    return fmaxf(amax * (1.f / 127.f), kTinyScale);
+  } else {
+    // amax = 1.m x 2^(e - 127): 448 = 1.75 x 2^8, so the exponent to divide by
+    // is e - 127 - 8, one more where 1.m > 1.75.
+    const uint32_t u = __builtin_bit_cast(uint32_t, amax);
+    int e = (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+    e = max(e, 1);
+    return __builtin_bit_cast(float, (uint32_t)e << 23);
+  }
+}
+
+// Four scaled values as four codes, nearest (ties to even), saturated.  NaN: code
+// 0 in int8 (which has none), NaN in e4m3.
+template <int CODE>
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+  if constexpr (CODE == kCodeI8) {
+    const float x[4] = {a, b, c, d};
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float y = x[i] == x[i] ? fminf(fmaxf(x[i], -127.f), 127.f) : 0.f;
+      w |= ((uint32_t)(int)__builtin_rintf(y) & 0xffu) << (8 * i);
+    }
+    return w;
+  } else {
+    auto sat = [](float y) { return y == y ? fminf(fmaxf(y, -448.f), 448.f) : y; };
+    uint32_t w = __builtin_amdgcn_cvt_pk_fp8_f32(sat(a), sat(b), 0, false);
+    return __builtin_amdgcn_cvt_pk_fp8_f32(sat(c), sat(d), w, true);
+  }
+}
+
+template <int CODE>
+__device__ __forceinline__ void decode4(uint32_t w, float (&x)[4]) {
+  if constexpr (CODE == kCodeI8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)((w >> (8 * i)) & 0xffu);
+  } else {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false);
+    const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+    x[0] = lo[0], x[1] = lo[1], x[2] = hi[0], x[3] = hi[1];
+  }
+}
+
+// Eight elements at p as fp32.
+template <class T>
+__device__ __forceinline__ void load8(const void* base, int64_t at, float (&x)[8]) {
+  if constexpr (std::is_same<T, float>::value) {
+    const f32x4* p = reinterpret_cast<const f32x4*>((const float*)base + at);
+    const f32x4 a = p[0], b = p[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+  } else {
+    const u32x4 a = ldg_b128_cached((const uint16_t*)base + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = a[i];
+      x[2 * i] = to_f32<T>((uint16_t)(w & 0xffffu));
+      x[2 * i + 1] = to_f32<T>((uint16_t)(w >> 16));
+    }
+  }
+}
+
+// Chunks of eight elements that a thread keeps in registers between the pass for
+// amax and the pass that writes codes; a block with more re-reads the rest.
+constexpr int kKeep = 8;
+
+template <class T, int CODE, int NT>
+__global__ void __launch_bounds__(NT) q8_append_kernel(Q8AppendParams p) {
+  __shared__ float red[NT / 64];
+  const int tid = threadIdx.x;
+  int item = blockIdx.x;
+  const int kv = item & 1;
+  item >>= 1;
+  const int h = item % p.Hkv;
+  item /= p.Hkv;
+  const int j = item % p.blocks;
+  const int b = item / p.blocks;
+  const int start = max(p.lens[b], 0);
+  const int n_new = p.news ? min(max(p.news[b], 0), p.T) : p.T;
+  if (n_new == 0 || start >= p.cap) return;
+  // Tokens [lo, lo + block) of the row; the new ones among them [a, z).
+  const int64_t lo = ((int64_t)start / p.block + j) * p.block;
+  const int64_t a = lo > start ? lo : start;
+  int64_t z = (int64_t)start + n_new;
+  z = z < p.cap ? z : p.cap;
+  z = z < lo + p.block ? z : lo + p.block;
+  if (a >= z) return;
+  int64_t unit = b, row = lo;
+  if (p.table) {
+    const int page = p.table[(int64_t)b * p.max_pages + (int)(lo / p.page_size)];
+    if (page < 0 || page >= p.num_pages) return;
+    unit = page;
+    row = lo % p.page_size;
+  }
+  const Q8Cache& c = p.c[kv];
+  uint8_t* codes = c.codes + unit * c.sb + (int64_t)h * c.sh + row * c.ss;
+  float* scale = c.scales + unit * c.cb + (int64_t)h * c.ch + (row / p.block) * c.cs;
+  const int older = (int)(a - lo);
+  const int cpr = p.D / 8;  // chunks per token
+  const int n = (int)(z - a) * cpr;
+  const int t0 = (int)(a - start);
+  const int half = p.D >> 1;
+
+  auto fetch = [&](int i, float (&x)[8]) SK_INLINE {
+    const int r = i / cpr;
+    const int d0 = (i - r * cpr) * 8;
+    const int64_t at = (int64_t)b * p.x_sb[kv] + (int64_t)h * p.x_sh[kv] + (int64_t)(t0 + r) * p.x_ss[kv];
+    load8<T>(p.x[kv], at + d0, x);
+    if (kv == 0) {
+      const int rr = rope_row(p.rope, b, t0 + r);
+      if (rr >= 0) {
+        float y[8], cs[8], sn[8];
+        load8<T>(p.x[kv], at + (d0 < half ? d0 + half : d0 - half), y);
+        rope_coeffs<8>(p.rope, rr, d0, cs, sn);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = rope_mix(x[e], y[e], d0 < half, cs[e], sn[e]);
+      }
+    }
+  };
+  float amax = 0.f;
+  auto widest = [&](const float (&x)[8]) SK_INLINE {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float y = fabsf(x[e]);
+      amax = y < __builtin_inff() ? fmaxf(amax, y) : amax;
+    }
+  };
+  float keep[kKeep][8];
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i)
+    if (tid + i * NT < n) {
+      fetch(tid + i * NT, keep[i]);
+      widest(keep[i]);
+    }
+  for (int i = tid + kKeep * NT; i < n; i += NT) {
+    float x[8];
+    fetch(i, x);
+    widest(x);
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+  if constexpr (NT > 64) {
+    if ((tid & 63) == 0) red[tid >> 6] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) amax = fmaxf(amax, red[w]);
+  }
+  const float need = needed_scale<CODE>(amax);
+  const float had = older > 0 ? *scale : 0.f;
+  const float now = older > 0 && had > need ? had : need;
+  const float inv = 1.f / now;
+  auto put = [&](int i, const float (&x)[8]) SK_INLINE {
+    const int r = i / cpr;
+    const int d0 = (i - r * cpr) * 8;
+    const u32x2 w = {
+        encode4<CODE>(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv),
+        encode4<CODE>(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv)};
+    *reinterpret_cast<u32x2*>(codes + (int64_t)(older + r) * c.ss + d0) = w;
+  };
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i)
+    if (tid + i * NT < n) put(tid + i * NT, keep[i]);
+  for (int i = tid + kKeep * NT; i < n; i += NT) {
+    float x[8];
+    fetch(i, x);
+    put(i, x);
+  }
+  if (older > 0 && had < now) {
+    const float f = had / now;
+    for (int i = tid; i < older * cpr; i += NT) {
+      const int r = i / cpr;
+      const int d0 = (i - r * cpr) * 8;
+      u32x2* at = reinterpret_cast<u32x2*>(codes + (int64_t)r * c.ss + d0);
+      u32x2 w = *at;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        float x[4];
+        decode4<CODE>(w[q], x);
+        w[q] = encode4<CODE>(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
+      }
+      *at = w;
+    }
+  }
+  if constexpr (NT > 64) __syncthreads();  // every thread has read the old scale
+  if (tid == 0) *scale = now;
+}
+
+template <class T, int CODE>
+static hipError_t append_tc(const Q8AppendParams& p, hipStream_t s) {
+  const int64_t items = (int64_t)p.B * p.blocks * p.Hkv * 2;
+  if (items == 0) return hipSuccess;
+  // One wave where a block's new elements fit its registers twice over.
+  const int64_t elems = (int64_t)(p.T < p.block ? p.T : p.block) * p.D;
+  if (elems <= 64 * 8 * kKeep)
+    hipLaunchKernelGGL((q8_append_kernel<T, CODE, 64>), dim3((unsigned)items), dim3(64), 0, s, p);
+  else
+    hipLaunchKernelGGL((q8_append_kernel<T, CODE, 256>), dim3((unsigned)items), dim3(256), 0, s, p);
+  return hipGetLastError();
+}
+
+template <int CODE>
+static hipError_t append_c(int dtype, const Q8AppendParams& p, hipStream_t s) {
+  if (dtype == SK_F32) return append_tc<float, CODE>(p, s);
+  if (dtype == SK_F16) return append_tc<F16, CODE>(p, s);
+  return append_tc<BF16, CODE>(p, s);
+}
+
+hipError_t launch_q8_append(int dtype, int code, const Q8AppendParams& p, hipStream_t s) {
+  return code == kCodeI8 ? append_c<kCodeI8>(dtype, p, s) : append_c<kCodeE4M3>(dtype, p, s);
+}
+
+// ---------------------------------------------------------------- page plan
+//
+// Rows that grow take pages from the front of the ring of free pages in row
+// order, rows that shrink put theirs behind its end in row order: two exclusive
+// prefix sums over the batch.  A workgroup sums the rows in front of its own by
+// itself (8 bytes a row, from the L2), so one launch needs no order among
+// workgroups.  The entries a call reads (table entries that rows hold, ring
+// entries in front of the old end) are not the ones it writes (entries past those
+// held, ring entries behind the end), and lengths and ring state go to buffers of
+// their own: a call with the same inputs gives the same outputs again.
+
+constexpr int kPlanThreads = 256;
+
+struct PlanRow {
+  int old_len, grow, po, pn, need, back;
+  bool fits;
+};
+
+__device__ __forceinline__ PlanRow plan_row(const PagePlanParams& p, int b) {
+  PlanRow r;
+  const int64_t cap = (int64_t)p.max_pages * p.page_size;
+  int64_t o = max(p.lens[b], 0);
+  o = o < cap ? o : cap;
+  const int d = min(p.news[b], p.T);
+  int64_t want = o + d;
+  want = want > 0 ? want : 0;
+  r.fits = want <= cap;
+  if (!r.fits) want = o;
+  r.old_len = (int)o;
+  r.grow = (int)(want - o);
+  r.po = (int)((o + p.page_size - 1) / p.page_size);
+  r.pn = (int)((want + p.page_size - 1) / p.page_size);
+  r.need = max(r.pn - r.po, 0);
+  r.back = max(r.po - r.pn, 0);
+  return r;
+}
+
+// Sum of x over the workgroup (all threads get it).
+__device__ __forceinline__ int block_sum(int x, int* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+  __syncthreads();
+  int s = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; ++w) s += red[w];
+  return s;
+}
+
+// Inclusive prefix sum of x over the workgroup's threads.
+__device__ __forceinline__ int block_scan(int x, int* red) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) red[wave] = x;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) x += red[w];
+  return x;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PagePlanParams p) {
+  __shared__ int red[kPlanThreads / 64];
+  __shared__ int s_old[kPlanThreads], s_grow[kPlanThreads], s_po[kPlanThreads], s_pn[kPlanThreads];
+  __shared__ int s_front[kPlanThreads], s_end[kPlanThreads];
+  const int tid = threadIdx.x;
+  const int b0 = blockIdx.x * p.rows_per_wg;
+  const int nb = min(p.rows_per_wg, p.B - b0);
+  int head = p.state[0] % p.N;
+  if (head < 0) head += p.N;
+  const int count = min(max(p.state[1], 0), p.N);
+
+  // Pages that the rows in front take and give back.
+  int need = 0, back = 0;
+  for (int b = tid; b < b0; b += kPlanThreads) {
+    const PlanRow r = plan_row(p, b);
+    need += r.need, back += r.back;
+  }
+  need = block_sum(need, red);
+  back = block_sum(back, red);
+
+  PlanRow r{};
+  if (tid < nb) r = plan_row(p, b0 + tid);
+  const int cum = need + block_scan(r.need, red);
+  const int end = back + block_scan(r.back, red);
+  const bool granted = r.need == 0 || cum <= count;
+  if (!granted) r.grow = 0, r.pn = r.po;
+  s_old[tid] = r.old_len, s_grow[tid] = r.grow, s_po[tid] = r.po, s_pn[tid] = r.pn;
+  s_front[tid] = cum - r.need;
+  s_end[tid] = end - r.back;
+  const int used = block_sum(granted ? r.need : 0, red);  // (a barrier for the arrays above too)
+
+  // Ring index i places behind the front.
+  auto ring_at = [&](int64_t i) { return (int)((head + i) % p.N); };
+
+  if (blockIdx.y == 0) {
+    if (tid < nb) p.lens_out[b0 + tid] = r.old_len + r.grow;
+    // Table entries of rows that grow, ring entries from rows that shrink: a wave
+    // takes a row at a time.
+    for (int i = tid >> 6; i < nb; i += kPlanThreads / 64) {
+      int* row = p.table + (int64_t)(b0 + i) * p.table_stride;
+      const int po = s_po[i], pn = s_pn[i];
+      for (int j = po + (tid & 63); j < pn; j += 64) row[j] = p.ring[ring_at((int64_t)s_front[i] + j - po)];
+      for (int j = pn + (tid & 63); j < po; j += 64) {
+        const int64_t at = (int64_t)count + s_end[i] + j - pn;
+        if (at < p.N) p.ring[ring_at(at)] = row[j];
+      }
+    }
+    if (b0 + nb == p.B) {
+      // The last rows' workgroup knows the sums.  Pages in front of it: all that
+      // was asked for, or what the granted rows took of it.
+      const int all_back = back + block_sum(r.back, red);
+      int taken = 0;
+      if (need <= count) {
+        taken = need + used;
+      } else {
+        // Some row in front was refused: the pages of those that were not.
+        int carry = 0;
+        for (int c0 = 0; c0 < b0; c0 += kPlanThreads) {
+          const int b = c0 + tid;
+          const int n = b < b0 ? plan_row(p, b).need : 0;
+          const int at = carry + block_scan(n, red);
+          taken += block_sum(at <= count ? n : 0, red);
+          carry = carry + block_sum(n, red);
+        }
+      }
+      if (tid == 0) {
+        p.state_out[0] = (int)(((int64_t)head + taken) % p.N);
+        p.state_out[1] = (int)min((int64_t)p.N, (int64_t)count - taken + all_back);
+      }
+    }
+  }
+
+  // Slots of this workgroup's rows and tokens.
+  const int c0 = blockIdx.y * p.toks_per_wg;
+  const int nc = min(p.toks_per_wg, p.T - c0);
+  for (int i = tid; i < nb * nc; i += kPlanThreads) {
+    const int q = i / nc;
+    const int t = c0 + i - q * nc;
+    int64_t slot = -1;
+    if (t < s_grow[q]) {
+      const int pos = s_old[q] + t;
+      const int j = pos / p.page_size;
+      const int page = j < s_po[q] ? p.table[(int64_t)(b0 + q) * p.table_stride + j]
+                                   : p.ring[ring_at((int64_t)s_front[q] + j - s_po[q])];
+      if (page >= 0) slot = (int64_t)page * p.page_size + (pos - j * p.page_size);
+    }
+    p.slots[(int64_t)(b0 + q) * p.T + t] = slot;
+  }
+}
+
+hipError_t launch_page_plan(const PagePlanParams& p0, hipStream_t s) {
+  PagePlanParams p = p0;
+  if (p.B == 0) return hipSuccess;
+  // About 2,048 slots a workgroup: whole rows while several fit, else parts of one.
+  const int64_t most = 2048;
+  p.rows_per_wg = (int)(p.T >= most ? 1 : p.T <= most / kPlanThreads ? kPlanThreads : most / p.T);
+  p.toks_per_wg = p.T < most ? (p.T > 0 ? p.T : 1) : (int)most;
+  const int64_t gx = (p.B + p.rows_per_wg - 1) / p.rows_per_wg;
+  const int64_t gy = p.T > 0 ? (p.T + p.toks_per_wg - 1) / p.toks_per_wg : 1;
+  if (gy > 65535) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL(page_plan_kernel, dim3((unsigned)gx, (unsigned)gy), dim3(kPlanThreads), 0, s, p);
+  return hipGetLastError();
+}
+
+}  // namespace sk

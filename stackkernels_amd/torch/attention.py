@@ -17,11 +17,14 @@ from typing import Any
 import torch
 import torch.nn as nn
 
+from stackkernels_amd._core.attention.attn_q8 import attention_q8, validate_q8_attention
 from stackkernels_amd._core.attention.decode import flash_decode as core_flash_decode
 from stackkernels_amd._core.attention.decode import flash_decode_paged as core_flash_decode_paged
 from stackkernels_amd._core.attention.flash_bwd import flash_attn_bwd
 from stackkernels_amd._core.attention._rope import rope_args, rope_rotate
 from stackkernels_amd._core.attention.flash_fwd import flash_attn_fwd
+from stackkernels_amd._core.cache.quantized import _integer, table_operand
+from stackkernels_amd._reference.torch import quantized
 from stackkernels_amd._reference.torch.attention import (
     attention_reference,
     attention_reference_backward,
@@ -292,6 +295,104 @@ def _decode_varlen_reference(q, k, v, sm_scale, cache_seqlens):
     return out
 
 
+def flash_attention_q8(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    is_causal: bool = False,
+    sm_scale: float | None = None,
+    cache_seqlens: torch.Tensor | None = None,
+    block_table: torch.Tensor | None = None,
+    query_lens: torch.Tensor | None = None,
+    *,
+    block_size: int = 32,
+    rope_cos: torch.Tensor | None = None,
+    rope_sin: torch.Tensor | None = None,
+    start_pos: int | torch.Tensor = 0,
+) -> torch.Tensor:
+    """Attention of S_q query tokens per row over a cache held in 8 bits.
+
+    For what a server computes against ``kv_cache_update_q8``'s cache: a chunk of a
+    prompt, a whole prompt behind a cached prefix, drafted tokens; ``flash_decode_q8``
+    is the form for one token.  The codes enter the matrix products as they are
+    (every one is exact in 16 bits) and the scales apply to float32 scores and
+    probabilities, so the cached values are not rounded again.  No gradients.
+
+    Args:
+        q: (B, H_q, S_q, D), bf16, fp16 or fp32; D a multiple of 16 up to 256.
+        k, v: codes, ``int8`` or ``float8_e4m3fn``, (B, H_kv, S_k, D) or page pools
+            (num_pages, H_kv, page_size, D); 16-byte-aligned rows, contiguous D.
+        k_scale, v_scale: float32 (B, H_kv, ceil(S_k / block_size)) or (num_pages,
+            H_kv, page_size / block_size).
+        is_causal: query i of a row with n keys and m queries sees keys ``j <= n - m
+            + i`` (bottom-right aligned); else all n.
+        sm_scale: score scale, default 1/sqrt(D).
+        cache_seqlens: integer (B,) keys per row, the new tokens' own included
+            (default S_k; required with block_table).
+        block_table: integer (B, max_pages) for a paged cache; keys in a page outside
+            the pool are left out.
+        query_lens: optional integer (B,): row b has ``query_lens[b]`` queries (the
+            first ones); the others give zeros, as does a query that sees no key.
+        block_size: tokens per scale, a multiple of 32 that divides page_size.
+        rope_cos, rope_sin, start_pos: rotate query i of row b to position
+            ``start_pos + i`` (typically ``start_pos=cache_seqlens - query_lens``).
+
+    Returns:
+        (B, H_q, S_q, D) in q's dtype.
+    """
+    if torch.is_grad_enabled() and q.requires_grad:
+        raise RuntimeError("attention over an 8-bit cache has no backward pass: call it under "
+                           "torch.no_grad() or on q.detach()")
+    if should_use_hip(q):
+        return attention_q8(q, k, v, k_scale, v_scale, is_causal, sm_scale, cache_seqlens,
+                            block_table, query_lens, block_size, rope_cos, rope_sin, start_pos)
+    _, _, _, sk, _ = validate_q8_attention(q, k, v, k_scale, v_scale, cache_seqlens, block_table,
+                                           query_lens, block_size)
+    b, _, sq, d = q.shape
+
+    def counts(x, name, most):
+        if x is None:
+            return [most] * b
+        return [min(max(n, 0), most) for n in _integer(x, name, (b,)).tolist()]
+
+    if rope_cos is not None or rope_sin is not None:
+        q = _rope_reference(q, rope_cos, rope_sin, start_pos)
+    table = None if block_table is None else table_operand(block_table, b).tolist()
+    return quantized.attention(q, k, v, k_scale, v_scale, counts(cache_seqlens, "cache_seqlens", sk),
+                               counts(query_lens, "query_lens", sq), table, block_size, is_causal,
+                               1.0 / math.sqrt(d) if sm_scale is None else sm_scale)
+
+
+def flash_decode_q8(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    sm_scale: float | None = None,
+    cache_seqlens: torch.Tensor | None = None,
+    block_table: torch.Tensor | None = None,
+    *,
+    block_size: int = 32,
+    rope_cos: torch.Tensor | None = None,
+    rope_sin: torch.Tensor | None = None,
+    start_pos: int | torch.Tensor = 0,
+) -> torch.Tensor:
+    """Decode of one query token (S_q = 1) over a cache held in 8 bits.
+
+    ``flash_decode`` over ``kv_cache_update_q8``'s cache: q (B, H_q, 1, D), the other
+    arguments as for ``flash_attention_q8`` (row b sees its first
+    ``cache_seqlens[b]`` keys; a row with no key gives zeros).  Returns (B, H_q, 1,
+    D) in q's dtype.
+    """
+    assert q.dim() != 4 or q.shape[2] == 1, f"flash_decode_q8 requires q_len == 1, got {q.shape[2]}"
+    return flash_attention_q8(q, k, v, k_scale, v_scale, False, sm_scale, cache_seqlens,
+                              block_table, None, block_size=block_size, rope_cos=rope_cos,
+                              rope_sin=rope_sin, start_pos=start_pos)
+
+
 class FlashAttention(nn.Module):
     """FlashAttention module with MHA, GQA and MQA support.
 
@@ -463,6 +564,8 @@ _register_decode_ops()
 __all__ = [
     "flash_attention",
     "flash_decode",
+    "flash_attention_q8",
+    "flash_decode_q8",
     "FlashAttention",
     "FlashAttentionFunction",
 ]
