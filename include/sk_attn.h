@@ -532,12 +532,27 @@ SK_API int sk_kv_page_plan(int32_t* block_table, const int32_t* cache_seqlens,
                     int num_free, void* stream);
 
 /*
+ * Sizes, types and strides of a call over an 8-bit cache (host memory, read during
+ * the call): a caller keeps one per shape.
+ */
+typedef struct {
+  int32_t dtype, code;          /* of the 16/32-bit tensors, of the codes */
+  int32_t B, Hq, Hkv, S;        /* S: new tokens (append) or query tokens; append: Hq unused */
+  int32_t units, rows;          /* B and S_cache, or num_pages and page_size */
+  int32_t max_pages;            /* 0: contiguous */
+  int32_t block_size, D, is_causal;
+  int64_t x_strides[2][3];      /* append: k, v; attention: q, o */
+  int64_t code_strides[2][3];   /* k and v codes */
+  int64_t scale_strides[2][3];  /* {unit, head, block} of their scales */
+} sk_q8_shape;
+
+/*
  * Append to a cache of 8-bit codes with one fp32 scale per block of block_size
  * tokens and KV head (an element's value is scale * code).  Token t < new_lens[b]
  * (NULL: T; clamped to [0, T]) of batch row b of k, v (B, Hkv, T, D) becomes
  * token max(cache_seqlens[b], 0) + t of row b.
  *
- * units = B, rows = S_cache, block_table NULL: the caches are (B, Hkv, S_cache,
+ * units = B, rows = S_cache, max_pages = 0: the caches are (B, Hkv, S_cache,
  * D), their scales (B, Hkv, ceil(S_cache / block_size)).  Else they are pools of
  * units pages of rows = page_size tokens with scales (units, Hkv, page_size /
  * block_size), token n of row b in page block_table[b, n / page_size] of (B,
@@ -557,17 +572,12 @@ SK_API int sk_kv_page_plan(int32_t* block_table, const int32_t* cache_seqlens,
  *
  * D: a multiple of 16 up to 256.  block_size: a multiple of 32 that divides
  * page_size.  Pointers to k, v and codes are 16-byte aligned, k, v strides
- * multiples of 8 elements (4 for fp32), code strides multiples of 16; scale
- * strides are int64_t[3] = {unit, head, block}.
+ * multiples of 8 elements (4 for fp32), code strides multiples of 16.
  */
-SK_API int sk_kv_cache_update_q8(int dtype, int code, const void* k, const void* v, void* k_cache,
+SK_API int sk_kv_cache_update_q8(const sk_q8_shape* shape, const void* k, const void* v, void* k_cache,
                           void* v_cache, float* k_scale, float* v_scale,
                           const int32_t* cache_seqlens, const int32_t* new_lens,
-                          const int32_t* block_table, int B, int Hkv, int T, int units, int rows,
-                          int max_pages, int block_size, int D, const int64_t* k_strides,
-                          const int64_t* v_strides, const int64_t* kc_strides,
-                          const int64_t* vc_strides, const int64_t* ks_strides,
-                          const int64_t* vs_strides, const void* rope_cos, const void* rope_sin,
+                          const int32_t* block_table, const void* rope_cos, const void* rope_sin,
                           int rope_dtype, int rope_rows, int64_t rope_stride,
                           const int32_t* rope_pos, int rope_start, void* stream);
 
@@ -595,16 +605,12 @@ SK_API int sk_attn_q8_plan(int dtype, int B, int Hq, int Hkv, int Sq, int Sk, in
  * 256, + 1) * 4 * B * Hq * Sq bytes per split when it is above 1.  Limits on D,
  * block_size, alignment and strides as above; a code row stride is 0 or at least D.
  */
-SK_API int sk_attn_q8(int dtype, int code, const void* q, const void* k_cache, const void* v_cache,
+SK_API int sk_attn_q8(const sk_q8_shape* shape, const void* q, const void* k_cache, const void* v_cache,
                const float* k_scale, const float* v_scale, void* o, void* workspace,
-               size_t workspace_bytes, int num_splits, int B, int Hq, int Hkv, int Sq, int units,
-               int rows, int max_pages, int block_size, int D, const int64_t* q_strides,
-               const int64_t* kc_strides, const int64_t* vc_strides, const int64_t* ks_strides,
-               const int64_t* vs_strides, const int64_t* o_strides, const int32_t* block_table,
-               const int32_t* cache_seqlens, const int32_t* query_lens, int is_causal,
-               const void* rope_cos, const void* rope_sin, int rope_dtype, int rope_rows,
-               int64_t rope_stride, const int32_t* rope_pos, int rope_start, float sm_scale,
-               void* stream);
+               size_t workspace_bytes, int num_splits, const int32_t* block_table,
+               const int32_t* cache_seqlens, const int32_t* query_lens, const void* rope_cos,
+               const void* rope_sin, int rope_dtype, int rope_rows, int64_t rope_stride,
+               const int32_t* rope_pos, int rope_start, float sm_scale, void* stream);
 
 #ifdef __cplusplus
 }

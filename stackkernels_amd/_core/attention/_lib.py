@@ -12,6 +12,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 import threading
 
 SK_F32, SK_F16, SK_BF16 = 0, 1, 2
@@ -102,16 +103,13 @@ SIGNATURES: dict[str, tuple] = {
                                                _i64p, _i64p, _i64p, _i64p, *_ROPE, _vp]),
     "sk_kv_page_plan": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int,
                                  ctypes.c_int64, _c_int, _c_int, _c_int, _vp]),
-    "sk_kv_cache_update_q8": (_c_int, [_c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
-                                       _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
-                                       _c_int, _i64p, _i64p, _i64p, _i64p, _i64p, _i64p, *_ROPE,
+    # (the first argument: an sk_q8_shape, see q8_shape)
+    "sk_kv_cache_update_q8": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, *_ROPE,
                                        _vp]),
     "sk_attn_q8_plan": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                  _intp, _sizep]),
-    "sk_attn_q8": (_c_int, [_c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t,
-                            _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
-                            _c_int, _c_int, _i64p, _i64p, _i64p, _i64p, _i64p, _i64p, _vp, _vp,
-                            _vp, _c_int, *_ROPE, _c_float, _vp]),
+    "sk_attn_q8": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _c_int, _vp,
+                            _vp, _vp, *_ROPE, _c_float, _vp]),
     "sk_kernel_config": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                   _c_int, _c_int, _c_int, _c_int, _i64p, ctypes.c_char_p,
                                   ctypes.c_size_t]),
@@ -193,6 +191,14 @@ def code_type(dtype) -> int:
         return SK_E4M3
     raise NotImplementedError(f"cache dtype {dtype} has no HIP kernel (supported: int8, "
                               "float8_e4m3fn)")
+
+
+_Q8_SHAPE = struct.Struct("=12i18q")
+
+
+def q8_shape(ints, strides) -> ctypes.Array:
+    """An ``sk_q8_shape``: its twelve sizes and six stride triples."""
+    return ctypes.create_string_buffer(_Q8_SHAPE.pack(*ints, *(n for st in strides for n in st)))
 
 
 def stream_ptr(device) -> int:

@@ -1047,24 +1047,26 @@ int sk_rope_rotate(int dtype, const void* x, void* out, int B, int H, int S, int
 // ---------------------------------------------------------------- 8-bit cache
 
 // The format's shape rules shared by the append and the attention.
-static int check_q8(int dtype, int code, int B, int Hkv, int units, int rows, int max_pages,
-                    bool paged, int block_size, int D) {
+static int check_q8(const sk_q8_shape* sh) {
+  if (!sh) return fail(SK_EINVAL, "shape pointer is NULL");
+  const int dtype = sh->dtype, code = sh->code, B = sh->B, Hkv = sh->Hkv, units = sh->units;
+  const int rows = sh->rows, max_pages = sh->max_pages, block_size = sh->block_size, D = sh->D;
   if (dtype != SK_F32 && dtype != SK_F16 && dtype != SK_BF16)
     return fail(SK_EUNSUPPORTED, "unsupported dtype code %d", dtype);
   if (code != SK_I8 && code != SK_E4M3)
     return fail(SK_EUNSUPPORTED, "unsupported code type %d (int8 or float8 e4m3)", code);
-  if (B < 0 || Hkv <= 0 || units < 0 || rows < 0 || max_pages < 0 || D <= 0)
-    return fail(SK_EINVAL, "invalid sizes B=%d Hkv=%d units=%d rows=%d max_pages=%d D=%d", B, Hkv,
-                units, rows, max_pages, D);
+  if (B < 0 || Hkv <= 0 || sh->S < 0 || units < 0 || rows < 0 || max_pages < 0 || D <= 0)
+    return fail(SK_EINVAL, "invalid sizes B=%d Hkv=%d S=%d units=%d rows=%d max_pages=%d D=%d", B,
+                Hkv, sh->S, units, rows, max_pages, D);
   if (D % 16 != 0 || D > 256)
     return fail(SK_EUNSUPPORTED, "head dim %d unsupported: need a multiple of 16 up to 256", D);
   if (block_size <= 0 || block_size % 32 != 0)
     return fail(SK_EINVAL, "block_size=%d must be a positive multiple of 32", block_size);
-  if (paged) {
+  if (max_pages > 0) {
     if (rows <= 0 || rows % block_size != 0)
       return fail(SK_EINVAL, "page_size=%d must be a positive multiple of block_size=%d", rows,
                   block_size);
-    if (max_pages > 0 && units == 0) return fail(SK_EINVAL, "empty page pool");
+    if (units == 0) return fail(SK_EINVAL, "empty page pool");
     if ((int64_t)max_pages * rows > 0x7fff0000LL)
       return fail(SK_EINVAL, "max_pages * page_size overflows int");
   } else if (units != B) {
@@ -1079,7 +1081,6 @@ static int check_q8(int dtype, int code, int B, int Hkv, int units, int rows, in
 // a row's last bytes would then read rows behind the visible ones).
 static int make_q8_cache(const char* name, const void* codes, const float* scales,
                          const int64_t* st, const int64_t* sst, int D, sk::Q8Cache* c) {
-  if (!st || !sst) return fail(SK_EINVAL, "%s strides pointer is NULL", name);
   for (int i = 0; i < 3; ++i) {
     if (st[i] < 0 || st[i] % 16 != 0)
       return fail(SK_EINVAL, "%s stride[%d]=%lld must be a non-negative multiple of 16 elements",
@@ -1150,25 +1151,25 @@ int sk_kv_page_plan(int32_t* block_table, const int32_t* cache_seqlens, const in
   return SK_OK;
 }
 
-int sk_kv_cache_update_q8(int dtype, int code, const void* k, const void* v, void* k_cache,
+int sk_kv_cache_update_q8(const sk_q8_shape* shape, const void* k, const void* v, void* k_cache,
                           void* v_cache, float* k_scale, float* v_scale,
                           const int32_t* cache_seqlens, const int32_t* new_lens,
-                          const int32_t* block_table, int B, int Hkv, int T, int units, int rows,
-                          int max_pages, int block_size, int D, const int64_t* k_strides,
-                          const int64_t* v_strides, const int64_t* kc_strides,
-                          const int64_t* vc_strides, const int64_t* ks_strides,
-                          const int64_t* vs_strides, const void* rope_cos, const void* rope_sin,
+                          const int32_t* block_table, const void* rope_cos, const void* rope_sin,
                           int rope_dtype, int rope_rows, int64_t rope_stride,
                           const int32_t* rope_pos, int rope_start, void* stream) {
   g_err[0] = 0;
-  const bool paged = block_table != nullptr || max_pages > 0;
-  int rc = check_q8(dtype, code, B, Hkv, units, rows, max_pages, paged, block_size, D);
+  int rc = check_q8(shape);
   if (rc) return rc;
-  if (T < 0) return fail(SK_EINVAL, "invalid T=%d", T);
+  const sk_q8_shape& sh = *shape;
+  const int B = sh.B, Hkv = sh.Hkv, T = sh.S, D = sh.D, rows = sh.rows;
+  const bool paged = sh.max_pages > 0;
   sk::Q8AppendParams p{};
-  if ((rc = check_strides(dtype, "k", k_strides)) || (rc = check_strides(dtype, "v", v_strides)) ||
-      (rc = make_q8_cache("k_cache", k_cache, k_scale, kc_strides, ks_strides, D, &p.c[0])) ||
-      (rc = make_q8_cache("v_cache", v_cache, v_scale, vc_strides, vs_strides, D, &p.c[1])))
+  if ((rc = check_strides(sh.dtype, "k", sh.x_strides[0])) ||
+      (rc = check_strides(sh.dtype, "v", sh.x_strides[1])) ||
+      (rc = make_q8_cache("k_cache", k_cache, k_scale, sh.code_strides[0], sh.scale_strides[0], D,
+                          &p.c[0])) ||
+      (rc = make_q8_cache("v_cache", v_cache, v_scale, sh.code_strides[1], sh.scale_strides[1], D,
+                          &p.c[1])))
     return rc;
   for (int i = 0; i < 2; ++i)
     if (rows > 1 && p.c[i].ss == 0) return fail(SK_EINVAL, "cache rows overlap (row stride 0)");
@@ -1177,7 +1178,7 @@ int sk_kv_cache_update_q8(int dtype, int code, const void* k, const void* v, voi
                         rope_start, D, B > 0 ? T : 0, &p.rope)))
       return rc;
   }
-  if ((int64_t)B * T == 0 || rows == 0 || (paged && max_pages == 0)) return SK_OK;
+  if ((int64_t)B * T == 0 || rows == 0) return SK_OK;
   if (paged && !block_table) return fail(SK_EINVAL, "block_table pointer is NULL");
   if ((rc = check_ptr("k", k)) || (rc = check_ptr("v", v)) || (rc = check_ptr("k_cache", k_cache)) ||
       (rc = check_ptr("v_cache", v_cache)))
@@ -1186,19 +1187,17 @@ int sk_kv_cache_update_q8(int dtype, int code, const void* k, const void* v, voi
     return fail(SK_EINVAL, "%s pointer is NULL",
                 !k_scale ? "k_scale" : !v_scale ? "v_scale" : "cache_seqlens");
   p.x[0] = k, p.x[1] = v;
-  for (int i = 0; i < 2; ++i) {
-    const int64_t* st = i ? v_strides : k_strides;
-    p.x_sb[i] = st[0], p.x_sh[i] = st[1], p.x_ss[i] = st[2];
-  }
+  for (int i = 0; i < 2; ++i)
+    p.x_sb[i] = sh.x_strides[i][0], p.x_sh[i] = sh.x_strides[i][1], p.x_ss[i] = sh.x_strides[i][2];
   p.lens = cache_seqlens, p.news = new_lens, p.table = paged ? block_table : nullptr;
   p.B = B, p.Hkv = Hkv, p.T = T, p.D = D;
-  p.cap = paged ? max_pages * rows : rows;
-  p.page_size = rows, p.max_pages = max_pages, p.num_pages = units;
-  p.block = block_size;
-  p.blocks = (int)(((int64_t)T + block_size - 2) / block_size + 1);
+  p.cap = paged ? sh.max_pages * rows : rows;
+  p.page_size = rows, p.max_pages = sh.max_pages, p.num_pages = sh.units;
+  p.block = sh.block_size;
+  p.blocks = (int)(((int64_t)T + p.block - 2) / p.block + 1);
   if ((int64_t)B * p.blocks * Hkv * 2 * 256 > 0xffffffffLL)
     return fail(SK_EINVAL, "grid too large: %d rows of %d new tokens, %d heads", B, T, Hkv);
-  const hipError_t e = sk::launch_q8_append(dtype, code, p, (hipStream_t)stream);
+  const hipError_t e = sk::launch_q8_append(sh.dtype, sh.code, p, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "sk_kv_cache_update_q8 launch");
   return SK_OK;
 }
@@ -1215,26 +1214,27 @@ int sk_attn_q8_plan(int dtype, int B, int Hq, int Hkv, int Sq, int Sk, int D, in
   return SK_OK;
 }
 
-int sk_attn_q8(int dtype, int code, const void* q, const void* k_cache, const void* v_cache,
+int sk_attn_q8(const sk_q8_shape* shape, const void* q, const void* k_cache, const void* v_cache,
                const float* k_scale, const float* v_scale, void* o, void* workspace,
-               size_t workspace_bytes, int num_splits, int B, int Hq, int Hkv, int Sq, int units,
-               int rows, int max_pages, int block_size, int D, const int64_t* q_strides,
-               const int64_t* kc_strides, const int64_t* vc_strides, const int64_t* ks_strides,
-               const int64_t* vs_strides, const int64_t* o_strides, const int32_t* block_table,
-               const int32_t* cache_seqlens, const int32_t* query_lens, int is_causal,
-               const void* rope_cos, const void* rope_sin, int rope_dtype, int rope_rows,
-               int64_t rope_stride, const int32_t* rope_pos, int rope_start, float sm_scale,
-               void* stream) {
+               size_t workspace_bytes, int num_splits, const int32_t* block_table,
+               const int32_t* cache_seqlens, const int32_t* query_lens, const void* rope_cos,
+               const void* rope_sin, int rope_dtype, int rope_rows, int64_t rope_stride,
+               const int32_t* rope_pos, int rope_start, float sm_scale, void* stream) {
   g_err[0] = 0;
-  const bool paged = block_table != nullptr || max_pages > 0;
-  int rc = check_q8(dtype, code, B, Hkv, units, rows, max_pages, paged, block_size, D);
+  int rc = check_q8(shape);
   if (rc) return rc;
-  const int Sk = paged ? max_pages * rows : rows;
+  const sk_q8_shape& sh = *shape;
+  const int dtype = sh.dtype, B = sh.B, Hq = sh.Hq, Hkv = sh.Hkv, Sq = sh.S, D = sh.D;
+  const bool paged = sh.max_pages > 0;
+  const int Sk = paged ? sh.max_pages * sh.rows : sh.rows;
   if ((rc = check_dims(dtype, B, Hq, Hkv, Sq, Sk, D))) return rc;
   sk::Q8AttnParams p{};
-  if ((rc = check_strides(dtype, "q", q_strides)) || (rc = check_strides(dtype, "o", o_strides)) ||
-      (rc = make_q8_cache("k_cache", k_cache, k_scale, kc_strides, ks_strides, D, &p.k)) ||
-      (rc = make_q8_cache("v_cache", v_cache, v_scale, vc_strides, vs_strides, D, &p.v)))
+  if ((rc = check_strides(dtype, "q", sh.x_strides[0])) ||
+      (rc = check_strides(dtype, "o", sh.x_strides[1])) ||
+      (rc = make_q8_cache("k_cache", k_cache, k_scale, sh.code_strides[0], sh.scale_strides[0], D,
+                          &p.k)) ||
+      (rc = make_q8_cache("v_cache", v_cache, v_scale, sh.code_strides[1], sh.scale_strides[1], D,
+                          &p.v)))
     return rc;
   if (rope_cos || rope_sin) {
     if ((rc = make_rope(rope_cos, rope_sin, rope_dtype, rope_rows, rope_stride, rope_pos,
@@ -1251,13 +1251,13 @@ int sk_attn_q8(int dtype, int code, const void* q, const void* k_cache, const vo
     return fail(SK_EINVAL, "block_table and cache_seqlens are required");
   if ((int64_t)Sq * (Hq / Hkv) > 0x7fff0000LL) return fail(SK_EINVAL, "Sq * group overflows int");
   p.q = q, p.o = o;
-  p.q_sb = q_strides[0], p.q_sh = q_strides[1], p.q_ss = q_strides[2];
-  p.o_sb = o_strides[0], p.o_sh = o_strides[1], p.o_ss = o_strides[2];
+  p.q_sb = sh.x_strides[0][0], p.q_sh = sh.x_strides[0][1], p.q_ss = sh.x_strides[0][2];
+  p.o_sb = sh.x_strides[1][0], p.o_sh = sh.x_strides[1][1], p.o_ss = sh.x_strides[1][2];
   p.B = B, p.Hq = Hq, p.Hkv = Hkv, p.Sq = Sq, p.Sk = Sk, p.D = D, p.group = Hq / Hkv;
   p.rows = Sq * p.group;
   if (num_splits == 0) num_splits = sk::q8_splits(dtype, B, Hkv, p.rows, Sk, D);
-  if (num_splits < 1 || num_splits > 1024)
-    return fail(SK_EINVAL, "num_splits=%d outside [1, 1024]", num_splits);
+  if (num_splits < 1 || num_splits > sk::kQ8MaxSplits)
+    return fail(SK_EINVAL, "num_splits=%d outside [1, %d]", num_splits, sk::kQ8MaxSplits);
   const size_t need = q8_ws_bytes(B, Hq, Sq, D, num_splits);
   if (need > 0 && (rc = check_ptr("workspace", workspace)))
     return fail(SK_EWORKSPACE, "workspace pointer is NULL or not 16-byte aligned");
@@ -1275,12 +1275,14 @@ int sk_attn_q8(int dtype, int code, const void* q, const void* k_cache, const vo
     p.part_o = (float*)workspace;
     p.part_lse = p.part_o + (size_t)B * Hq * Sq * num_splits * p.dpad;
   }
-  p.causal = is_causal != 0;
-  p.block = block_size;
+  p.causal = sh.is_causal != 0;
+  p.dtype = dtype;
+  p.block_div = sk::FastDiv(sh.block_size);
+  if (paged) p.page_div = sk::FastDiv(sh.rows);
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.seqlens = cache_seqlens, p.qlens = query_lens, p.table = paged ? block_table : nullptr;
-  p.page_size = rows, p.max_pages = max_pages, p.num_pages = units;
-  const hipError_t e = sk::launch_q8_attn(dtype, code, p, (hipStream_t)stream);
+  p.page_size = sh.rows, p.max_pages = sh.max_pages, p.num_pages = sh.units;
+  const hipError_t e = sk::launch_q8_attn(sh.code, p, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "sk_attn_q8 launch");
   return SK_OK;
 }

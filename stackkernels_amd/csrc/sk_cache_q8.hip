@@ -251,61 +251,65 @@ hipError_t launch_q8_append(int dtype, int code, const Q8AppendParams& p, hipStr
 // their own: a call with the same inputs gives the same outputs again.
 
 constexpr int kPlanThreads = 256;
+constexpr int kPlanWaves = kPlanThreads / 64;
 
 struct PlanRow {
   int old_len, grow, po, pn, need, back;
-  bool fits;
 };
+
+__device__ __forceinline__ int pages_of(const PagePlanParams& p, int n) {
+  const int q = p.page_div.quot(n);
+  return q + (q * p.page_size != n);
+}
 
 __device__ __forceinline__ PlanRow plan_row(const PagePlanParams& p, int b) {
   PlanRow r;
-  const int64_t cap = (int64_t)p.max_pages * p.page_size;
-  int64_t o = max(p.lens[b], 0);
-  o = o < cap ? o : cap;
-  const int d = min(p.news[b], p.T);
-  int64_t want = o + d;
-  want = want > 0 ? want : 0;
-  r.fits = want <= cap;
-  if (!r.fits) want = o;
-  r.old_len = (int)o;
-  r.grow = (int)(want - o);
-  r.po = (int)((o + p.page_size - 1) / p.page_size);
-  r.pn = (int)((want + p.page_size - 1) / p.page_size);
+  const int cap = p.max_pages * p.page_size;  // (below 2^31: checked on the host)
+  const int o = min(max(p.lens[b], 0), cap);
+  int64_t want = (int64_t)o + min(p.news[b], p.T);
+  want = want < 0 ? 0 : want > cap ? o : want;
+  r.old_len = o;
+  r.grow = (int)want - o;
+  r.po = pages_of(p, o);
+  r.pn = pages_of(p, (int)want);
   r.need = max(r.pn - r.po, 0);
   r.back = max(r.po - r.pn, 0);
   return r;
 }
 
-// Sum of x over the workgroup (all threads get it).
-__device__ __forceinline__ int block_sum(int x, int* red) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
-  __syncthreads();
-  int s = 0;
-#pragma unroll
-  for (int w = 0; w < kPlanThreads / 64; ++w) s += red[w];
-  return s;
-}
-
-// Inclusive prefix sum of x over the workgroup's threads.
-__device__ __forceinline__ int block_scan(int x, int* red) {
+// Inclusive prefix sums of x and y over the workgroup's threads; totals in tx, ty.
+__device__ __forceinline__ void block_scan2(int& x, int& y, int& tx, int& ty,
+                                            int (&red)[2][kPlanWaves]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o);
-    if (lane >= o) x += y;
+    const int u = __shfl_up(x, o), v = __shfl_up(y, o);
+    if (lane >= o) x += u, y += v;
+  }
+  if (lane == 63) red[0][wave] = x, red[1][wave] = y;
+  __syncthreads();
+  tx = ty = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanWaves; ++w) {
+    if (w == wave) x += tx, y += ty;
+    tx += red[0][w], ty += red[1][w];
   }
   __syncthreads();
-  if (lane == 63) red[wave] = x;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) x += red[w];
-  return x;
+}
+
+// Last of n ascending numbers that is at most i (the first one is).
+__device__ __forceinline__ int last_at_most(const int* v, int n, int i) {
+  int lo = 0;
+  while (n > 1) {
+    const int h = n >> 1;
+    if (v[lo + h] <= i) lo += h, n -= h;
+    else n = h;
+  }
+  return lo;
 }
 
 __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PagePlanParams p) {
-  __shared__ int red[kPlanThreads / 64];
+  __shared__ int red[2][kPlanWaves];
   __shared__ int s_old[kPlanThreads], s_grow[kPlanThreads], s_po[kPlanThreads], s_pn[kPlanThreads];
   __shared__ int s_front[kPlanThreads], s_end[kPlanThreads];
   const int tid = threadIdx.x;
@@ -314,64 +318,74 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PagePlanParams 
   int head = p.state[0] % p.N;
   if (head < 0) head += p.N;
   const int count = min(max(p.state[1], 0), p.N);
+  PlanRow r{};
+  if (tid < nb) r = plan_row(p, b0 + tid);
 
   // Pages that the rows in front take and give back.
   int need = 0, back = 0;
-  for (int b = tid; b < b0; b += kPlanThreads) {
-    const PlanRow r = plan_row(p, b);
-    need += r.need, back += r.back;
+  if (b0 > 0) {
+    for (int b = tid; b < b0; b += kPlanThreads) {
+      const PlanRow f = plan_row(p, b);
+      need += f.need, back += f.back;
+    }
+    int tx, ty;
+    block_scan2(need, back, tx, ty, red);
+    need = tx, back = ty;
   }
-  need = block_sum(need, red);
-  back = block_sum(back, red);
-
-  PlanRow r{};
-  if (tid < nb) r = plan_row(p, b0 + tid);
-  const int cum = need + block_scan(r.need, red);
-  const int end = back + block_scan(r.back, red);
-  const bool granted = r.need == 0 || cum <= count;
+  int cum = r.need, end = r.back, all_need, all_back;
+  block_scan2(cum, end, all_need, all_back, red);
+  const bool granted = r.need == 0 || need + cum <= count;
   if (!granted) r.grow = 0, r.pn = r.po;
   s_old[tid] = r.old_len, s_grow[tid] = r.grow, s_po[tid] = r.po, s_pn[tid] = r.pn;
   s_front[tid] = cum - r.need;
   s_end[tid] = end - r.back;
-  const int used = block_sum(granted ? r.need : 0, red);  // (a barrier for the arrays above too)
+  __syncthreads();
 
-  // Ring index i places behind the front.
-  auto ring_at = [&](int64_t i) { return (int)((head + i) % p.N); };
+  // Ring place i behind the front (0 <= i < N).
+  auto ring_at = [&](int i) SK_INLINE {
+    const uint32_t at = (uint32_t)head + (uint32_t)i;
+    return at >= (uint32_t)p.N ? at - (uint32_t)p.N : at;
+  };
 
   if (blockIdx.y == 0) {
     if (tid < nb) p.lens_out[b0 + tid] = r.old_len + r.grow;
-    // Table entries of rows that grow, ring entries from rows that shrink: a wave
-    // takes a row at a time.
-    for (int i = tid >> 6; i < nb; i += kPlanThreads / 64) {
-      int* row = p.table + (int64_t)(b0 + i) * p.table_stride;
-      const int po = s_po[i], pn = s_pn[i];
-      for (int j = po + (tid & 63); j < pn; j += 64) row[j] = p.ring[ring_at((int64_t)s_front[i] + j - po)];
-      for (int j = pn + (tid & 63); j < po; j += 64) {
-        const int64_t at = (int64_t)count + s_end[i] + j - pn;
-        if (at < p.N) p.ring[ring_at(at)] = row[j];
-      }
+    // Pages taken by rows that grow, page by page over the workgroup's rows.
+    for (int i = tid; i < all_need && need + i < count; i += kPlanThreads) {
+      const int q = last_at_most(s_front, kPlanThreads, i);
+      const int j = s_po[q] + i - s_front[q];
+      if (j < s_pn[q])  // (a refused row has no new pages)
+        p.table[(int64_t)(b0 + q) * p.table_stride + j] = p.ring[ring_at(need + i)];
+    }
+    // Pages given back by rows that shrink.
+    for (int i = tid; i < all_back; i += kPlanThreads) {
+      const int q = last_at_most(s_end, kPlanThreads, i);
+      const int64_t at = (int64_t)count + back + i;
+      if (at < p.N)
+        p.ring[ring_at((int)at)] = p.table[(int64_t)(b0 + q) * p.table_stride + s_pn[q] + i - s_end[q]];
     }
     if (b0 + nb == p.B) {
-      // The last rows' workgroup knows the sums.  Pages in front of it: all that
-      // was asked for, or what the granted rows took of it.
-      const int all_back = back + block_sum(r.back, red);
-      int taken = 0;
-      if (need <= count) {
-        taken = need + used;
-      } else {
-        // Some row in front was refused: the pages of those that were not.
+      // Pages taken in all: those up to the last row that was granted some, which
+      // is in front of this workgroup's where their sum exceeds the ring's.
+      int taken = granted && r.need > 0 ? need + cum : need <= count ? need : 0;
+      if (need > count) {
         int carry = 0;
         for (int c0 = 0; c0 < b0; c0 += kPlanThreads) {
           const int b = c0 + tid;
-          const int n = b < b0 ? plan_row(p, b).need : 0;
-          const int at = carry + block_scan(n, red);
-          taken += block_sum(at <= count ? n : 0, red);
-          carry = carry + block_sum(n, red);
+          int x = b < b0 ? plan_row(p, b).need : 0, y = 0, tx, ty;
+          block_scan2(x, y, tx, ty, red);
+          if (carry + x <= count) taken = max(taken, carry + x);
+          carry += tx;
         }
       }
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) taken = max(taken, __shfl_xor(taken, o));
+      if ((tid & 63) == 0) red[0][tid >> 6] = taken;
+      __syncthreads();
       if (tid == 0) {
-        p.state_out[0] = (int)(((int64_t)head + taken) % p.N);
-        p.state_out[1] = (int)min((int64_t)p.N, (int64_t)count - taken + all_back);
+#pragma unroll
+        for (int w = 1; w < kPlanWaves; ++w) taken = max(taken, red[0][w]);
+        p.state_out[0] = (int)ring_at(taken < p.N ? taken : 0);
+        p.state_out[1] = (int)min((int64_t)p.N, (int64_t)count - taken + back + all_back);
       }
     }
   }
@@ -380,14 +394,14 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PagePlanParams 
   const int c0 = blockIdx.y * p.toks_per_wg;
   const int nc = min(p.toks_per_wg, p.T - c0);
   for (int i = tid; i < nb * nc; i += kPlanThreads) {
-    const int q = i / nc;
+    const int q = p.rows_per_wg == 1 ? 0 : p.tok_div.quot(i);  // (several rows: all T tokens)
     const int t = c0 + i - q * nc;
     int64_t slot = -1;
     if (t < s_grow[q]) {
       const int pos = s_old[q] + t;
-      const int j = pos / p.page_size;
+      const int j = p.page_div.quot(pos);
       const int page = j < s_po[q] ? p.table[(int64_t)(b0 + q) * p.table_stride + j]
-                                   : p.ring[ring_at((int64_t)s_front[q] + j - s_po[q])];
+                                   : p.ring[ring_at(need + s_front[q] + j - s_po[q])];
       if (page >= 0) slot = (int64_t)page * p.page_size + (pos - j * p.page_size);
     }
     p.slots[(int64_t)(b0 + q) * p.T + t] = slot;
@@ -401,6 +415,8 @@ hipError_t launch_page_plan(const PagePlanParams& p0, hipStream_t s) {
   const int64_t most = 2048;
   p.rows_per_wg = (int)(p.T >= most ? 1 : p.T <= most / kPlanThreads ? kPlanThreads : most / p.T);
   p.toks_per_wg = p.T < most ? (p.T > 0 ? p.T : 1) : (int)most;
+  p.page_div = FastDiv(p.page_size);
+  p.tok_div = FastDiv(p.T > 0 ? p.T : 1);
   const int64_t gx = (p.B + p.rows_per_wg - 1) / p.rows_per_wg;
   const int64_t gy = p.T > 0 ? (p.T + p.toks_per_wg - 1) / p.toks_per_wg : 1;
   if (gy > 65535) return hipErrorInvalidConfiguration;

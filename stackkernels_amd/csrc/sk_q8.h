@@ -17,6 +17,26 @@ namespace sk {
 constexpr int kCodeI8 = 3;
 constexpr int kCodeE4M3 = 4;
 
+// Quotients by a fixed positive number of 0 <= n < 2^31: floor(n / d) = high word of
+// n * mul, shifted, with mul = floor(2^(32 + shift) / d) + 1 and 2^shift the
+// largest power of two below d (d > 1): the error n (mul d - 2^(32 + shift)) <= n d
+// stays below 2^(32 + shift).
+struct FastDiv {
+  uint32_t mul;
+  int shift;
+  FastDiv() = default;
+  explicit FastDiv(int d) {
+    shift = 0;
+    while ((2LL << shift) < d) ++shift;
+    mul = d <= 1 ? 0 : (uint32_t)((1ULL << (32 + shift)) / (uint64_t)d + 1);
+  }
+  __device__ __forceinline__ int quot(int n) const {
+    return mul ? (int)(__umulhi((uint32_t)n, mul) >> shift) : n;
+  }
+};
+
+constexpr int kQ8MaxSplits = 256;
+
 // One cache (k or v) as the kernels address it: strides in elements.
 struct Q8Cache {
   uint8_t* codes;
@@ -37,7 +57,8 @@ struct PagePlanParams {
   int* lens_out;
   int* state_out;
   int B, max_pages, page_size, T, N;
-  int rows_per_wg, toks_per_wg;
+  int rows_per_wg, toks_per_wg;  // whole rows (toks_per_wg = T), or parts of one
+  FastDiv page_div, tok_div;
 };
 
 // Quantising append: token t < news[b] of batch row b becomes token
@@ -71,18 +92,19 @@ struct Q8AttnParams {
   int rows, row_blocks;
   int num_splits, dpad;
   int causal;
-  int block;
+  int dtype;             // of q and o
   float scale_log2;      // sm_scale * log2(e), signed
   const int* seqlens;    // null: Sk
   const int* qlens;      // null: Sq
   const int* table;      // null: contiguous
   int page_size, max_pages, num_pages;
+  FastDiv block_div, page_div;
   RopeParams rope;
 };
 
 hipError_t launch_page_plan(const PagePlanParams& p, hipStream_t s);
 hipError_t launch_q8_append(int dtype, int code, const Q8AppendParams& p, hipStream_t s);
-hipError_t launch_q8_attn(int dtype, int code, const Q8AttnParams& p, hipStream_t s);
+hipError_t launch_q8_attn(int code, const Q8AttnParams& p, hipStream_t s);
 // Rows of a KV head (query tokens x group) that one workgroup takes, and the
 // split count for a shape (keys: the most keys a row can see).
 int q8_rows_per_block(int dtype, int D, int rows);

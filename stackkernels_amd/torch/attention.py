@@ -17,13 +17,17 @@ from typing import Any
 import torch
 import torch.nn as nn
 
-from stackkernels_amd._core.attention.attn_q8 import attention_q8, validate_q8_attention
+from stackkernels_amd._core.attention.attn_q8 import (
+    attention_q8,
+    table_width,
+    validate_q8_attention,
+)
 from stackkernels_amd._core.attention.decode import flash_decode as core_flash_decode
 from stackkernels_amd._core.attention.decode import flash_decode_paged as core_flash_decode_paged
 from stackkernels_amd._core.attention.flash_bwd import flash_attn_bwd
 from stackkernels_amd._core.attention._rope import rope_args, rope_rotate
 from stackkernels_amd._core.attention.flash_fwd import flash_attn_fwd
-from stackkernels_amd._core.cache.quantized import _integer, table_operand
+from stackkernels_amd._core.cache.quantized import _integer, layout_of, table_operand
 from stackkernels_amd._reference.torch import quantized
 from stackkernels_amd._reference.torch.attention import (
     attention_reference,
@@ -348,8 +352,9 @@ def flash_attention_q8(
     if should_use_hip(q):
         return attention_q8(q, k, v, k_scale, v_scale, is_causal, sm_scale, cache_seqlens,
                             block_table, query_lens, block_size, rope_cos, rope_sin, start_pos)
-    _, _, _, sk, _ = validate_q8_attention(q, k, v, k_scale, v_scale, cache_seqlens, block_table,
-                                           query_lens, block_size)
+    width = table_width(q, cache_seqlens, block_table)
+    sk = validate_q8_attention(*(layout_of(t) for t in (q, k, v, k_scale, v_scale)), width,
+                               block_size)[3]
     b, _, sq, d = q.shape
 
     def counts(x, name, most):

@@ -12,10 +12,15 @@ import torch
 
 from stackkernels_amd._core.cache.kv_update import kv_cache_update as _core_kv_cache_update
 from stackkernels_amd._core.cache.kv_update import validate_cache_update
-from stackkernels_amd._core.cache.quantized import _integer, table_operand, validate_page_plan
+from stackkernels_amd._core.cache.quantized import (
+    _integer,
+    layout_of,
+    table_operand,
+    validate_page_plan,
+    validate_q8_update,
+)
 from stackkernels_amd._core.cache.quantized import kv_cache_update_q8 as _core_kv_cache_update_q8
 from stackkernels_amd._core.cache.quantized import kv_page_plan as _core_kv_page_plan
-from stackkernels_amd._core.cache.quantized import validate_q8_update
 from stackkernels_amd._reference.torch import quantized
 from stackkernels_amd.torch._dispatch import should_use_hip
 
@@ -136,8 +141,9 @@ def kv_cache_update_q8(
         _core_kv_cache_update_q8(k, v, k_cache, v_cache, k_scale, v_scale, cache_seqlens, new_lens,
                                  block_table, block_size, rope_cos, rope_sin, start_pos)
         return
-    b, _, t, _, _, _ = validate_q8_update(k, v, k_cache, v_cache, k_scale, v_scale, block_table,
-                                          block_size)
+    b, _, t, _, _, _ = validate_q8_update(
+        *(layout_of(x) for x in (k, v, k_cache, v_cache, k_scale, v_scale)),
+        block_table is not None, block_size)
     lens = _integer(cache_seqlens, "cache_seqlens", (b,)).tolist()
     news = [t] * b if new_lens is None else _integer(new_lens, "new_lens", (b,)).tolist()
     table = None if block_table is None else table_operand(block_table, b).tolist()

@@ -44,37 +44,50 @@ def rotate64(x, cos, sin, pos):
     return out
 
 
-def attention64(q, kc, vc, ks, vs, block, lens, q_lens, table, causal, scale, splits=1):
+def attention64(q, kc, vc, ks, vs, block, lens, q_lens, table, causal, scale, splits=1, dtype=None,
+                rotated=False):
     """(output, bound) in float64 on the CPU.  The bound counts, for each output
-    element: the rounding of the probabilities to q's type and that of the result
-    (u each, relative), the fp32 score (D + 16 roundings of a product sum and a
-    few of the exponent, each 2^-23 of the sum of magnitudes), the fp32 sums over
-    the keys, and for fp16 the subnormal probabilities (2^-25 each)."""
+    element o = sum p_n t_n c_n (u: half a step, relative, of q's type):
+
+    * the result's rounding, u |o| (and 2^-25 where fp16 results are subnormal);
+    * the probabilities' rounding to fp16, 2^-11 p_n each, or to the sum of two fp16
+      numbers for fp32 queries, 2^-22 (the second one's 2^-11 of the first one's
+      2^-11), and at least 2^-25 of the largest p_j t_j, the step of subnormals in
+      the kernel's units;
+    * the queries' rounding in the same way (rotated 16-bit ones, all fp32 ones; the
+      others are exact down to 2^-25 of their row's largest element), which moves a
+      score by as much of sum |q_d| |k_d| and a probability by twice that;
+    * the fp32 scores: D + 16 roundings of the product's sum and a few of the
+      exponent, 2^-23 each, likewise; and the fp32 sums over the keys.
+    """
     b, hq, sq, d = q.shape
     hkv = kc.shape[1]
-    u = U[q.dtype]
+    dtype = q.dtype if dtype is None else dtype
+    u = U[dtype]
+    two = 2.0 ** -22 if dtype == torch.float32 else 2.0 ** -11
+    u_q = two if rotated or dtype == torch.float32 else 0.0
     out = torch.zeros(b, hq, sq, d, dtype=torch.float64)
     tol = torch.zeros_like(out)
     for i in range(b):
         n, m = lens[i], q_lens[i]
         if table is None:
-            k, v = values64(kc[i], ks[i], block)[:, :n], values64(vc[i], vs[i], block)[:, :n]
+            k, c = values64(kc[i], ks[i], block)[:, :n], vc[i].float().double()[:, :n]
+            t = vs[i].double().repeat_interleave(block, dim=-1)[:, :n]
             at = torch.arange(n)
         else:
             page = kc.shape[2]
-            at, ku, vu = [], [], []
+            at, ku, cu, tu = [], [], [], []
             for j in range(n):
-                p = table[i][j // page]
+                p, r = table[i][j // page], j % page
                 if 0 <= p < kc.shape[0]:
                     at.append(j)
-                    ku.append(kc[p, :, j % page].float().double()
-                              * ks[p, :, j % page // block].double()[:, None])
-                    vu.append(vc[p, :, j % page].float().double()
-                              * vs[p, :, j % page // block].double()[:, None])
+                    ku.append(kc[p, :, r].float().double() * ks[p, :, r // block].double()[:, None])
+                    cu.append(vc[p, :, r].float().double())
+                    tu.append(vs[p, :, r // block].double())
             if not at:
                 continue
             at = torch.tensor(at)
-            k, v = torch.stack(ku, 1), torch.stack(vu, 1)
+            k, c, t = torch.stack(ku, 1), torch.stack(cu, 1), torch.stack(tu, 1)
         if n == 0 or m == 0:
             continue
         for h in range(hq):
@@ -82,20 +95,21 @@ def attention64(q, kc, vc, ks, vs, block, lens, q_lens, table, causal, scale, sp
             x = q[i, h, :m].double()
             s = x @ k[g].T * scale
             mag = (x.abs() @ k[g].abs().T * abs(scale)).amax(-1, keepdim=True)
+            edge = x.abs().amax(-1, keepdim=True) * k[g].abs().sum(-1).amax() * abs(scale)
             if causal:
                 s = s.masked_fill(at[None] > torch.arange(n - m, n)[:, None], -math.inf)
             top = s.amax(-1, keepdim=True)
             e = torch.exp(s - torch.where(top == -math.inf, 0.0, top))
-            total = e.sum(-1, keepdim=True).clamp(min=1e-300)
-            p = e / total
-            out[i, h, :m] = p @ v[g]
-            mean = p @ v[g].abs()
-            rel = u + 2 * ((d + 16) * 2.0 ** -23 * mag + 2.0 ** -21) + (n + splits) * 2.0 ** -23
-            tol[i, h, :m] = (rel * mean + u * out[i, h, :m].abs()) * 1.0 + 1e-30
-            if q.dtype == torch.float16:
-                # Below 2^-14 fp16 steps by 2^-24 whatever the size, so there a rounding
-                # is off by at most 2^-25: of each probability, and of the result.
-                tol[i, h, :m] += 2.0 ** -25 * v[g].abs().sum(0) / total + 2.0 ** -25
+            p = e / e.sum(-1, keepdim=True).clamp(min=1e-300)
+            w = p * t[g]
+            o, mean = w @ c[g], w @ c[g].abs()
+            rel = (two + 2 * ((u_q + (d + 16) * 2.0 ** -23) * mag + 2.0 ** -25 * edge + 2.0 ** -21)
+                   + (n + splits) * 2.0 ** -23)
+            out[i, h, :m] = o
+            tol[i, h, :m] = (rel * mean + u * o.abs() + 1e-30
+                             + 2.0 ** -25 * w.amax(-1, keepdim=True) * c[g].abs().sum(0))
+            if dtype == torch.float16:
+                tol[i, h, :m] += 2.0 ** -25
     return out, tol
 
 

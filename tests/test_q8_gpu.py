@@ -182,16 +182,11 @@ def _attend(dtype, code, hq, hkv, sq, d, block, page, lens, q_lens=None, causal=
     if rope:
         cos, sin = precompute_freqs(d, cap + sq + 1)
         starts = [max(n - m, 0) for n, m in zip(lens, ql)]
-        qr = q.clone()
-        for i in range(b):
-            qr[i] = _q8.rotate64(q[i].double(), cos, sin, starts[i]).to(dtype)
+        qr = torch.stack([_q8.rotate64(q[i].double(), cos, sin, starts[i]) for i in range(b)])
         kw = dict(rope_cos=cos.cuda(), rope_sin=sin.cuda(), start_pos=i32(starts))
     want, tol = _q8.attention64(qr, kc, vc, ks, vs, block, lens, ql,
                                 None if table is None else table.tolist(), causal, sc,
-                                splits or 1)
-    if rope:  # the rotated q's own rounding may differ by a step where the sums tie
-        u = _q8.U[dtype]
-        tol = tol + 2 * u * 2 * want.abs().amax() + 4 * u
+                                splits or 1, dtype, rope)
     # Every code and scale behind the rows' lengths is NaN on the device.
     dk, dv, dks, dvs = (x.clone().cuda() for x in (kc, vc, ks, vs))
     if poison:
