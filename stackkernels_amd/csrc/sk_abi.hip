@@ -1080,7 +1080,8 @@ static int check_q8(const sk_q8_shape* sh) {
 // Code and scale strides -> c.  Rows of codes may not overlap in part (a load of
 // a row's last bytes would then read rows behind the visible ones).
 static int make_q8_cache(const char* name, const void* codes, const float* scales,
-                         const int64_t* st, const int64_t* sst, int D, sk::Q8Cache* c) {
+                         const int64_t* st, const int64_t* sst, int D, bool paged,
+                         sk::Q8Cache* c) {
   for (int i = 0; i < 3; ++i) {
     if (st[i] < 0 || st[i] % 16 != 0)
       return fail(SK_EINVAL, "%s stride[%d]=%lld must be a non-negative multiple of 16 elements",
@@ -1092,8 +1093,15 @@ static int make_q8_cache(const char* name, const void* codes, const float* scale
   if (st[2] != 0 && st[2] < D)
     return fail(SK_EINVAL, "%s row stride %lld is less than the head dim %d", name,
                 (long long)st[2], D);
-  if (st[2] > (1LL << 25))
+  // (The kernels' tiles span less than 2^31 bytes; pages and scales are addressed by
+  // products of 32-bit numbers.)
+  if (st[2] > (1LL << 23))
     return fail(SK_EINVAL, "%s row stride %lld is too large", name, (long long)st[2]);
+  for (int i = 0; i < 3; ++i)
+    if (st[i] > 0xffffffffLL && paged)
+      return fail(SK_EINVAL, "%s stride[%d]=%lld is too large", name, i, (long long)st[i]);
+    else if (sst[i] > 0x7fffffffLL)
+      return fail(SK_EINVAL, "%s scale stride[%d]=%lld is too large", name, i, (long long)sst[i]);
   c->codes = (uint8_t*)const_cast<void*>(codes);
   c->scales = const_cast<float*>(scales);
   c->sb = st[0], c->sh = st[1], c->ss = st[2];
@@ -1167,9 +1175,9 @@ int sk_kv_cache_update_q8(const sk_q8_shape* shape, const void* k, const void* v
   if ((rc = check_strides(sh.dtype, "k", sh.x_strides[0])) ||
       (rc = check_strides(sh.dtype, "v", sh.x_strides[1])) ||
       (rc = make_q8_cache("k_cache", k_cache, k_scale, sh.code_strides[0], sh.scale_strides[0], D,
-                          &p.c[0])) ||
+                          paged, &p.c[0])) ||
       (rc = make_q8_cache("v_cache", v_cache, v_scale, sh.code_strides[1], sh.scale_strides[1], D,
-                          &p.c[1])))
+                          paged, &p.c[1])))
     return rc;
   for (int i = 0; i < 2; ++i)
     if (rows > 1 && p.c[i].ss == 0) return fail(SK_EINVAL, "cache rows overlap (row stride 0)");
@@ -1232,9 +1240,9 @@ int sk_attn_q8(const sk_q8_shape* shape, const void* q, const void* k_cache, con
   if ((rc = check_strides(dtype, "q", sh.x_strides[0])) ||
       (rc = check_strides(dtype, "o", sh.x_strides[1])) ||
       (rc = make_q8_cache("k_cache", k_cache, k_scale, sh.code_strides[0], sh.scale_strides[0], D,
-                          &p.k)) ||
+                          paged, &p.k)) ||
       (rc = make_q8_cache("v_cache", v_cache, v_scale, sh.code_strides[1], sh.scale_strides[1], D,
-                          &p.v)))
+                          paged, &p.v)))
     return rc;
   if (rope_cos || rope_sin) {
     if ((rc = make_rope(rope_cos, rope_sin, rope_dtype, rope_rows, rope_stride, rope_pos,

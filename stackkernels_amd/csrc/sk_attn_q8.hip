@@ -29,6 +29,7 @@
 //   columns VB m + c, so the transposition V^T needs is a byte selection.
 // The four waves of a workgroup take tiles in turn and merge their sums in LDS.
 #include <type_traits>
+#include <utility>
 
 #include "sk_common.h"
 #include "sk_q8.h"
@@ -136,8 +137,113 @@ __device__ __forceinline__ Q8Span q8_span(const Q8AttnParams& p, int b, int row0
   return s;
 }
 
-constexpr int kQ8Waves = 4;
+// f(0), f(1), ..., f(N - 1) with compile-time arguments.
+template <class F, int... I>
+__device__ __forceinline__ void static_for_impl(F& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void static_for(F f) {
+  static_for_impl(f, std::make_integer_sequence<int, N>{});
+}
+
 constexpr float kMinFactor = 1e-35f;  // of a score: keeps a masked -inf a -inf
+
+// How a tile's scores x (log2 units) become probabilities of one row: e = 2^(x +
+// offset) are the fp16 operands, in units of 2^m2; to_l takes their sum to the units
+// of l.  lost: the tile's V scale is so small (or 0) next to others that its operands
+// are all 0 in fp16; offset is then -inf, and l takes the sum of 2^(x + l_offset).
+struct Q8Weight {
+  float offset, to_l, l_offset;
+  bool lost;
+};
+
+// Running references of one row: m of the scores x, m2 of x + log2 t (t: the V
+// scale), l = sum of 2^(x - m).  -inf while no key was seen.
+struct Q8Ref {
+  float m = kNegInf, m2 = kNegInf, l = 0.f;
+  // mt, mt2: the tile's maxima.  True for a wave where some row's references rise,
+  // by more than kRescaleLog2 (smaller excesses only make e larger than 1): ao is
+  // then the factor of the row's sums.
+  __device__ __forceinline__ bool raise(float mt, float mt2, float& ao) {
+    if (!__any(mt > m + kRescaleLog2 || mt2 > m2 + kRescaleLog2)) return false;
+    const float m_new = fmaxf(m, mt), m2_new = fmaxf(m2, mt2);
+    l *= m_new == kNegInf ? 1.f : fast_exp2(m - m_new);
+    ao = m2_new == kNegInf ? 1.f : fast_exp2(m2 - m2_new);
+    m = m_new, m2 = m2_new;
+    return true;
+  }
+  // lv: log2 of the tile's V scale.  (A row that has seen no key has only -inf
+  // scores, whose e is 0 for any finite offset.)
+  __device__ __forceinline__ Q8Weight weight(float lv) const {
+    const float ms = m == kNegInf ? 0.f : m, m2s = m2 == kNegInf ? 0.f : m2;
+    Q8Weight w;
+    const float lw = lv + ms - m2s;  // log2 of an operand of a score m
+    w.lost = lw < -90.f;
+    w.offset = w.lost ? kNegInf : lv - m2s;
+    w.to_l = w.lost ? 1.f : fast_exp2(-lw);
+    w.l_offset = -ms;
+    return w;
+  }
+};
+
+// The query row of a lane as matrix operands: k-step s takes the eight columns from
+// col(s), divided by 2^(exponent of the row's largest element), which is spread
+// over the lanes that reduce() joins.  Returns the row's score factor.
+template <int KS, int TERMS, class Col, class Reduce>
+__device__ __forceinline__ float q8_query(const Q8AttnParams& p, int b, int hkv, int r, int ql,
+                                          Col col, Reduce reduce, u32x4 (&out)[KS][TERMS]) {
+  const int half = p.D >> 1;
+  const int t = r / p.group;
+  const bool live = r < p.rows && t < ql;
+  const int64_t at = live ? (int64_t)b * p.q_sb + (int64_t)(hkv * p.group + r - t * p.group) * p.q_sh +
+                                (int64_t)t * p.q_ss
+                          : 0;
+  const int rr = rope_row(p.rope, b, t);
+  float x[KS][8];
+  float top = 0.f;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int d0 = col(s);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[s][e] = 0.f;
+    if (live && d0 < p.D) load_q8x8(p.q, p.dtype, at + d0, x[s]);
+  }
+  if (rr >= 0) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d0 = col(s);
+      if (live && d0 < p.D) {
+        float y[8], cs[8], sn[8];
+        load_q8x8(p.q, p.dtype, at + (d0 < half ? d0 + half : d0 - half), y);
+        rope_coeffs<8>(p.rope, rr, d0, cs, sn);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[s][e] = rope_mix(x[s][e], y[e], d0 < half, cs[e], sn[e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[s][e]));
+  top = reduce(top);
+  int ex = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
+  if (ex > 127) ex = 0;  // an infinity: the row's scores are not finite anyway
+  const float sign = p.scale_log2 < 0.f ? -1.f : 1.f;
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t u[TERMS];
+      split2<TERMS>(sign * __builtin_amdgcn_ldexpf(x[s][2 * i], -ex),
+                    sign * __builtin_amdgcn_ldexpf(x[s][2 * i + 1], -ex), u);
+#pragma unroll
+      for (int k = 0; k < TERMS; ++k) out[s][k][i] = u[k];
+    }
+  return __builtin_amdgcn_ldexpf(fabsf(p.scale_log2), ex);
+}
+
+constexpr int kQ8Waves = 4;
 
 // Column blocks whose queries are read from LDS each tile (the four waves share
 // them): with more than 32 head-dim-128 columns the sums alone take 128
@@ -263,62 +369,19 @@ __global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams 
   u32x4 qreg[kQLds ? 1 : NC][KS][TERMS];
   float qmul[NC];
   if (k_lo < k_hi) {
-    const int half = p.D >> 1;
+    auto col = [&](int s) SK_INLINE { return 64 * (s >> 1) + 16 * g + 8 * (s & 1); };
+    auto reduce = [](float x) SK_INLINE { return xhalf_max(fmaxf(x, __shfl_xor(x, 16))); };
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      if (kQLds && c % NW != wave) continue;
       const int r = row0 + 16 * c + c16;
-      const int t = r / p.group;
-      const bool live = r < p.rows && t < sp.ql;
-      const int64_t at = live ? (int64_t)b * p.q_sb + (int64_t)(hkv * p.group + r - t * p.group) * p.q_sh +
-                                    (int64_t)t * p.q_ss
-                              : 0;
-      const int rr = rope_row(p.rope, b, t);
-      float x[KS][8];
-      float top = 0.f;
+      if constexpr (kQLds) {
+        if (c % NW != wave) continue;
+        qmul_s[c][lane] = q8_query<KS, TERMS>(p, b, hkv, r, sp.ql, col, reduce, qreg[0]);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int d0 = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[s][e] = 0.f;
-        if (live && d0 < p.D) {
-          load_q8x8(p.q, p.dtype, at + d0, x[s]);
-          if (rr >= 0) {
-            float y[8], cs[8], sn[8];
-            load_q8x8(p.q, p.dtype, at + (d0 < half ? d0 + half : d0 - half), y);
-            rope_coeffs<8>(p.rope, rr, d0, cs, sn);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[s][e] = rope_mix(x[s][e], y[e], d0 < half, cs[e], sn[e]);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[s][e]));
-      }
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = xhalf_max(top);
-      int ex = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
-      if (ex > 127) ex = 0;  // an infinity: the row's scores are not finite anyway
-      qmul[c] = __builtin_amdgcn_ldexpf(fabsf(p.scale_log2), ex);
-      const float sign = p.scale_log2 < 0.f ? -1.f : 1.f;
-      if (kQLds) qmul_s[kQLds ? c : 0][lane] = qmul[c];
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        u32x4 w[TERMS];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t u[TERMS];
-          split2<TERMS>(sign * __builtin_amdgcn_ldexpf(x[s][2 * i], -ex),
-                        sign * __builtin_amdgcn_ldexpf(x[s][2 * i + 1], -ex), u);
-#pragma unroll
-          for (int k = 0; k < TERMS; ++k) w[k][i] = u[k];
-        }
-#pragma unroll
-        for (int k = 0; k < TERMS; ++k) {
-          if constexpr (kQLds)
-            qs[(c * KS + s) * TERMS + k][lane] = w[k];
-          else
-            qreg[c][s][k] = w[k];
-        }
+        for (int i = 0; i < KS * TERMS; ++i)
+          qs[c * KS * TERMS + i][lane] = qreg[0][i / TERMS][i % TERMS];
+      } else {
+        qmul[c] = q8_query<KS, TERMS>(p, b, hkv, r, sp.ql, col, reduce, qreg[c]);
       }
     }
     if constexpr (kQLds) {
@@ -329,14 +392,11 @@ __global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams 
   }
 
   f32x4 oacc[NC][VB];
-  // Per column: -m (0 while there is no key), m, m2, l, and 2^(m - m2).
-  float m_neg[NC], m_run[NC], m2_run[NC], l_run[NC], w_run[NC];
+  Q8Ref ref[NC];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    m_run[c] = m2_run[c] = kNegInf, m_neg[c] = 0.f, l_run[c] = 0.f, w_run[c] = 0.f;
+  for (int c = 0; c < NC; ++c)
 #pragma unroll
     for (int i = 0; i < VB; ++i) oacc[c][i] = f32x4{};
-  }
 
   for (; n0 < k_hi; n0 += 32 * NW) {
     const float ks = ks_t, vs = vs_t;
@@ -392,27 +452,25 @@ __global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams 
                        fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
       mt = fmaxf(mt, __shfl_xor(mt, 16));
       mt = xhalf_max(mt) * mul;
-      const float mt2 = mt + lv;
-      if (__any(mt > m_run[c] + kRescaleLog2 || mt2 > m2_run[c] + kRescaleLog2)) {
-        const float m_new = fmaxf(m_run[c], mt), m2_new = fmaxf(m2_run[c], mt2);
-        const float al = m_new == kNegInf ? 1.f : fast_exp2(m_run[c] - m_new);
-        const float ao = m2_new == kNegInf ? 1.f : fast_exp2(m2_run[c] - m2_new);
-        m_run[c] = m_new, m2_run[c] = m2_new;
-        m_neg[c] = m_new == kNegInf ? 0.f : -m_new;
-        w_run[c] = m2_new == kNegInf ? 0.f : fast_exp2(m_new - m2_new);
-        l_run[c] *= al;
+      float ao;
+      if (ref[c].raise(mt, mt + lv, ao)) {
 #pragma unroll
         for (int i = 0; i < VB; ++i) oacc[c][i] *= ao;
       }
-      const float wv = vs * w_run[c];
+      const Q8Weight w = ref[c].weight(lv);
+      if (__any(w.lost)) {
+        float ps = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ps += fast_exp2(fmaf(e[i], mul, w.l_offset));
+        ref[c].l += w.lost ? ps : 0.f;
+      }
       float ps = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        e[i] = fast_exp2(fmaf(e[i], mul, m_neg[c]));
+        e[i] = fast_exp2(fmaf(e[i], mul, w.offset));
         ps += e[i];
-        e[i] *= wv;
       }
-      l_run[c] += ps;
+      ref[c].l += ps * w.to_l;
 #pragma unroll
       for (int i = 0; i < 4; ++i) split2<TERMS>(e[2 * i], e[2 * i + 1], pk[c][i]);
     }
@@ -447,10 +505,10 @@ __global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams 
   // M) and l by 2^(m - M), added in wave order.
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    float l = l_run[c] + __shfl_xor(l_run[c], 16);
+    float l = ref[c].l + __shfl_xor(ref[c].l, 16);
     l = xhalf_sum(l);
     if (g == 0) {
-      red_m[wave][16 * c + c16] = m_run[c];
+      red_m[wave][16 * c + c16] = ref[c].m;
       red_l[wave][16 * c + c16] = l;
     }
   }
@@ -460,7 +518,7 @@ __global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams 
     float mm = red_m[0][16 * c + c16];
 #pragma unroll
     for (int w = 1; w < NW; ++w) mm = fmaxf(mm, red_m[w][16 * c + c16]);
-    const float f = mm == kNegInf || m2_run[c] == kNegInf ? 1.f : fast_exp2(m2_run[c] - mm);
+    const float f = mm == kNegInf || ref[c].m2 == kNegInf ? 1.f : fast_exp2(ref[c].m2 - mm);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -495,7 +553,7 @@ __global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams 
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[e] = live ? s[e] * inv : 0.f;
           if (p.num_splits > 1)
-            *reinterpret_cast<f32x4*>(p.part_o + row * p.dpad + d0 + i) = f32x4{x[0], x[1], x[2], x[3]};
+            *reinterpret_cast<f32x4*>(p.part_o + row * DP + d0 + i) = f32x4{x[0], x[1], x[2], x[3]};
           else if (d0 + i < p.D)
             store_o4(p.o, p.dtype, at + i, x);
         }
@@ -507,6 +565,421 @@ __global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams 
     }
     __syncthreads();
   }
+}
+
+// Many rows: a workgroup of eight waves takes 256 rows of a KV head, 32 per wave,
+// and shares each tile of 8192 / DP keys, whose codes it widens to fp16 once, in
+// LDS.  S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16_f16.
+// * Pipeline: the body of a 32-key part u multiplies S(u + 1) and O += V(u) P(u), one
+//   MFMA a slot, and spreads over those slots the softmax of part u and a share of
+//   the widening: during tile t, K(t + 2) and then V(t + 1) go from registers into
+//   the LDS buffer that the tile before has read (three for K, two for V, one barrier
+//   a tile); the codes after those are loaded as the registers fall free.  Each slot
+//   is fenced, so the matrix unit waits for no long stretch of other work.
+// * V is widened in columns: a thread takes four columns of four keys and writes
+//   four rows of V^T, the keys in the order in which a lane of S^T's result holds
+//   them (0-3, 8-11 | 4-7, 12-15 of each 16).
+// * Rows of K and V^T are padded by 16 bytes: the 16 rows of an operand read lie in
+//   distinct banks.  A wave writes V^T in 16 rows four apart, 16 bytes each; chunk c
+//   of row d stands at c ^ (d / 16 % 4), which spreads those too, is the same for the
+//   16 rows of a read and, for a lane, one register and constants.  (Without it the
+//   writes made 45% of the LDS cycles conflicts.)
+// * Page ids and scales come through vector loads a tile or more ahead: scalar ones
+//   would make every LDS wait wait for them.
+// Against the kernel above a code is widened once per 256 rows, not per 32.
+template <int DP>
+struct Q8Big {
+  static constexpr int BN = 8192 / DP;   // keys per tile
+  static constexpr int NH = BN / 32;     // 32-key parts, each with its own scales
+  static constexpr int KSTR = DP + 8;    // fp16 per K row
+  static constexpr int VSTR = BN + 8;    // fp16 per V^T row
+};
+
+constexpr int kQ8BigWaves = 8;
+constexpr int kQ8BigRows = 32 * kQ8BigWaves;
+
+// PARTS: pages a tile may lie in (1: contiguous caches, pages of whole tiles).
+template <class C, int DP, bool PAGED, int PARTS>
+__global__ void __launch_bounds__(kQ8BigWaves * 64) q8_big_kernel(Q8AttnParams p) {
+  using L = Q8Big<DP>;
+  constexpr int NT = kQ8BigWaves * 64;
+  constexpr int BN = L::BN, NH = L::NH, KSTR = L::KSTR, VSTR = L::VSTR;
+  constexpr int PK = BN / PARTS;  // keys per part with an address of its own
+  constexpr int KS = DP / 16;     // k-steps of S^T
+  constexpr int DB = DP / 32;     // output blocks
+  constexpr int CPK = DP / 16;    // 16-byte pieces of a K row's codes: one per thread
+  constexpr int DC = DP / 4;      // 4-byte pieces of a V row's codes
+  static_assert(BN * CPK == NT && BN / 4 * DC == NT, "one piece of K and four of V per thread");
+  __shared__ __attribute__((aligned(16))) uint16_t ksm[3][BN * KSTR];
+  __shared__ __attribute__((aligned(16))) uint16_t vsm[2][DP * VSTR];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c32 = lane & 31;
+  const int hi2 = lane >> 5;
+
+  int item = xcd_work_index(blockIdx.x, gridDim.x);
+  const int rb = p.row_blocks - 1 - item % p.row_blocks;  // (causal: longest first)
+  item /= p.row_blocks;
+  const int split = item % p.num_splits;
+  item /= p.num_splits;
+  const int hkv = item % p.Hkv;
+  const int b = item / p.Hkv;
+
+  const int row0 = rb * kQ8BigRows;
+  const Q8Span sp = q8_span(p, b, row0, kQ8BigRows);
+  const int kps = ((sp.hi + p.num_splits - 1) / p.num_splits + BN - 1) / BN * BN;
+  const int k_lo = split * kps;
+  const int k_hi = min(sp.hi, k_lo + kps);
+  const int n_tiles = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
+  const int r = row0 + 32 * wave + c32;
+  const int t = r / p.group;
+  const int lim = min(p.causal ? sp.len - sp.ql + t + 1 : sp.len, k_hi);
+  // Tiles this wave's rows see, and keys that all of them see.
+  const int w0 = row0 + 32 * wave;
+  int w_tiles = 0, w_full = sp.len;
+  if (w0 < p.rows && w0 / p.group < sp.ql) {
+    const int last = min((min(w0 + 32, p.rows) - 1) / p.group, sp.ql - 1);
+    const int w_hi = p.causal ? min(sp.len - sp.ql + last + 1, k_hi) : k_hi;
+    w_tiles = w_hi > k_lo ? (w_hi - k_lo + BN - 1) / BN : 0;
+    if (p.causal) w_full = sp.len - sp.ql + w0 / p.group + 1;
+  }
+
+  // Where the codes of this KV head start (contiguous caches: of this row's too).
+  const int64_t unit0 = PAGED ? 0 : b;
+  const uint8_t* const kbase = p.k.codes + unit0 * p.k.sb + (int64_t)hkv * p.k.sh;
+  const uint8_t* const vbase = p.v.codes + unit0 * p.v.sb + (int64_t)hkv * p.v.sh;
+  const uint32_t ksb = (uint32_t)p.k.sb, vsb = (uint32_t)p.v.sb;  // (paged: below 2^32)
+  const uint32_t kss = (uint32_t)p.k.ss, vss = (uint32_t)p.v.ss;
+
+  // Lane j < 2 NH reads the scale of part j % NH: k's below NH, v's from there.
+  const int spart = lane % NH;
+  // Page of the lane's part of tile it (any page past the last key's).
+  const buf_rsrc table = make_rsrc(PAGED ? p.table + (int64_t)b * p.max_pages : nullptr,
+                                   PAGED ? p.max_pages * 4 : 0);
+  auto lane_key = [&](int it) SK_INLINE { return min(k_lo + it * BN + 32 * spart, k_hi - 1); };
+  auto load_page = [&](int it) SK_INLINE {
+    if constexpr (!PAGED) return 0;
+    return (int)__builtin_amdgcn_raw_buffer_load_b32(table, (uint32_t)p.page_div.quot(lane_key(it)) * 4, 0, 0);
+  };
+  auto settled_page = [&](int page) SK_INLINE {
+    return PARTS == 1 ? __builtin_amdgcn_readfirstlane(page) : page;
+  };
+  auto in_pool = [&](int page) SK_INLINE { return !PAGED || (page >= 0 && page < p.num_pages); };
+  auto load_scale = [&](int it, int page) SK_INLINE {
+    const int n = lane_key(it);
+    const int row = PAGED ? n - p.page_div.quot(n) * p.page_size : n;
+    const uint32_t unit = PAGED ? (in_pool(page) ? (uint32_t)page : 0u) : (uint32_t)b;
+    const uint32_t blk = (uint32_t)p.block_div.quot(row);
+    const bool is_v = lane / NH % 2;
+    const float* const base = is_v ? p.v.scales + (int64_t)hkv * p.v.ch : p.k.scales + (int64_t)hkv * p.k.ch;
+    return base[(uint64_t)unit * (uint32_t)(is_v ? p.v.cb : p.k.cb) +
+                (uint64_t)blk * (uint32_t)(is_v ? p.v.cs : p.k.cs)];
+  };
+  // Resource of part h of tile it: its keys below k_hi, none past the last tile or
+  // in a page outside the pool.
+  auto part_rsrc = [&](const uint8_t* base, uint32_t sb, uint32_t ss, int it, int h, int page) SK_INLINE {
+    const int n = k_lo + it * BN + h * PK;
+    int rows = max(min(PK, k_hi - n), 0);
+    uint64_t at = (uint64_t)(uint32_t)n * ss;
+    if constexpr (PAGED) {
+      const int pg = PARTS == 1 ? page : __builtin_amdgcn_readlane(page, h * (NH / PARTS));
+      rows = in_pool(pg) ? rows : 0;
+      at = (uint64_t)(in_pool(pg) ? (uint32_t)pg : 0u) * sb +
+           (uint64_t)(uint32_t)(n - p.page_div.quot(n) * p.page_size) * ss;
+    }
+    return make_rsrc(base + at, rows > 0 ? (rows - 1) * (int)ss + p.D : 0);
+  };
+
+  u32x4 kraw;
+  uint32_t vraw[4];
+  const int krow = tid / CPK, kcol = 16 * (tid % CPK);
+  const int kpart = PARTS == 1 ? 0 : __builtin_amdgcn_readfirstlane(krow / PK);
+  const uint32_t koff = kcol < p.D ? (uint32_t)((krow & (PK - 1)) * (int)kss + kcol) : kBufferOob;
+  // The thread's V: positions 4 vq .. 4 vq + 3, keys vkey .. vkey + 3 of the tile.
+  const int vq = 4 * (wave / (DC / 16)) + lane / 16, vcol = 64 * (wave % (DC / 16)) + 4 * (lane % 16);
+  const int vkey = 16 * (vq >> 2) + 8 * (vq & 1) + 4 * (vq >> 1 & 1);
+  const int vpart = PARTS == 1 ? 0 : __builtin_amdgcn_readfirstlane(vkey / PK);
+  const uint32_t voff = vcol < p.D ? (uint32_t)((vkey & (PK - 1)) * (int)vss + vcol) : kBufferOob;
+  auto load_k = [&](int it, int page) SK_INLINE {
+    kraw = buffer_load_b128(part_rsrc(kbase, ksb, kss, it, kpart, page), koff);
+  };
+  auto load_v = [&](int it, int page) SK_INLINE {
+    const buf_rsrc rs = part_rsrc(vbase, vsb, vss, it, vpart, page);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      vraw[e] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rs, voff, e * (int)vss, 0);
+  };
+  // Widening in steps, into buffer offsets kb and vb (fp16): K in eight (two codes
+  // each), V in four (two keys' two columns).
+  u32x4 kw;
+  u32x2 vw[2];
+  uint16_t* const kto = &ksm[0][krow * KSTR + kcol];
+  uint16_t* const vto = &vsm[0][vcol * VSTR + 8 * ((vq >> 1) ^ (vcol / 16 % 4)) + 4 * (vq & 1)];
+  auto widen_k = [&](int kb, auto step) SK_INLINE {
+    constexpr int st = decltype(step)::value;
+    kw[st & 3] = widen2<C, (st & 1)>(kraw[st >> 1]);
+    if constexpr ((st & 3) == 3) *reinterpret_cast<u32x4*>(kto + kb + 2 * (st - 3)) = kw;
+  };
+  auto widen_v = [&](int vb, auto step) SK_INLINE {
+    constexpr int st = decltype(step)::value, hf = st >> 1, i = st & 1;
+    uint32_t c0, c1;
+    widen_cols<C, hf>(vraw[2 * i], vraw[2 * i + 1], c0, c1);
+    vw[0][i] = c0, vw[1][i] = c1;
+    if constexpr (i == 1) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) *reinterpret_cast<u32x2*>(vto + vb + (2 * hf + c) * VSTR) = vw[c];
+    }
+  };
+
+  u32x4 q[KS][1];
+  f32x16 oacc[DB];
+#pragma unroll
+  for (int i = 0; i < DB; ++i) oacc[i] = f32x16{};
+  Q8Ref ref;
+  float qmul = 0.f;
+  // Scales of tile t's parts, settled when t is next: k's, and log2 of v's (0 and
+  // -inf: no such page); ok: parts whose page lies in the pool.
+  float ks_t[NH], lv_t[NH];
+  uint32_t ok_t = 0;
+  auto settle_scales = [&](float sv, int page) SK_INLINE {
+    sv = in_pool(page) ? sv : 0.f;
+    const float lv = __builtin_amdgcn_logf(sv);  // log2
+    ok_t = (1u << NH) - 1;
+    if constexpr (PAGED) {
+      if constexpr (PARTS == 1)
+        ok_t = in_pool(page) ? ok_t : 0u;
+      else
+        ok_t &= (uint32_t)__ballot(in_pool(page));
+    }
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      ks_t[h] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sv), h));
+      lv_t[h] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, lv), NH + h));
+    }
+  };
+
+  // Of the part whose scores are next: factor, operand offset, factor of the sum.
+  float mul = 0.f, off = 0.f, to_l = 0.f;
+  // Mask the scores of part h of the tile at n0 where some are hidden (mx: their raw
+  // maximum), raise the references.
+  auto settle = [&](int n0, auto part, f32x16& sc, float mx) SK_INLINE {
+    constexpr int h = decltype(part)::value;
+    const bool ok = ok_t >> h & 1;
+    if (!ok || n0 + 32 * h + 32 > w_full || n0 + 32 * h + 32 > k_hi) {
+      const int end = (ok ? lim : 0) - n0 - 32 * h - 4 * hi2;
+      mx = kNegInf;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if (8 * (i >> 2) + (i & 3) >= end) sc[i] = kNegInf;
+        mx = fmaxf(mx, sc[i]);
+      }
+    }
+    mul = fmaxf(ks_t[h] * qmul, kMinFactor);
+    mx = xhalf_max(mx) * mul;
+    float ao;
+    if (ref.raise(mx, mx + lv_t[h], ao)) {
+#pragma unroll
+      for (int i = 0; i < DB; ++i) oacc[i] *= ao;
+    }
+    const Q8Weight w = ref.weight(lv_t[h]);
+    off = w.offset, to_l = w.to_l;
+    if (__any(w.lost)) {
+      float ps = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ps += fast_exp2(fmaf(sc[i], mul, w.l_offset));
+      ref.l += w.lost ? ps : 0.f;
+    }
+  };
+
+  constexpr int NS = KS;        // score MFMAs of a part
+  constexpr int NO = 2 * DB;    // output MFMAs
+  constexpr int NM = NS + NO;
+  constexpr int NG = 8;         // pairs of scores a lane holds
+  constexpr int KLEAD = 4, OLEAD = 6;  // MFMAs an operand is read ahead of its own
+  constexpr int FL = NS + DB - 4;  // first slot of the last pair
+  constexpr int KST = 16 / NH, VST = 8 / NH;  // widening steps of a body that has some
+  static_assert(FL > 0 && NM >= KST && NM >= VST, "slots");
+
+  const uint16_t* const kfrom = &ksm[0][c32 * KSTR + 8 * hi2];
+  const uint16_t* const vfrom = &vsm[0][c32 * VSTR + 8 * (hi2 ^ (c32 / 16))];
+
+  // Body of part h (scores sc) of a tile: kr, vr: buffer offsets of the next part's
+  // tile in K and of this tile in V; kb, vb: of the tiles being widened.  nx: the
+  // next part's scores, mx their raw maximum.  kNow, kNext: this wave sees this
+  // part's tile, the next part's.
+  auto body = [&](auto part, auto now, auto next, int kr, int vr, int kb, int vb, const f32x16& sc,
+                  f32x16& nx, float& mx) SK_INLINE {
+    constexpr bool kNow = decltype(now)::value, kNext = decltype(next)::value;
+    constexpr int h = decltype(part)::value, hn = (h + 1) % NH;
+    u32x4 a[NS], vt[NO], pk[2];
+    float y[2 * NG], e[2 * NG], ps = 0.f;
+    auto read_k = [&](int i) SK_INLINE { return lds_read_b128(kfrom + kr + hn * 32 * KSTR + 16 * i); };
+    auto read_v = [&](int j) SK_INLINE {
+      const int blk = j % DB;  // (rows 32 blk + c32: chunk 4 h + 2 (j / DB) + hi2)
+      return lds_read_b128(vfrom + vr + blk * 32 * VSTR + 32 * h + 16 * (j / DB ^ blk % 2));
+    };
+    mx = kNegInf;
+    if constexpr (kNext) {
+#pragma unroll
+      for (int i = 0; i < KLEAD; ++i) a[i] = read_k(i);
+      nx = f32x16{};
+    }
+    static_for<NM>([&](auto ic) SK_INLINE {
+      constexpr int i = decltype(ic)::value;
+      if constexpr (kNext && i + KLEAD < NS) a[i + KLEAD] = read_k(i + KLEAD);
+      if constexpr (kNow && i + OLEAD >= NS && i + OLEAD - NS < NO)
+        vt[i + OLEAD - NS] = read_v(i + OLEAD - NS);
+      if constexpr (i < NS) {
+        if constexpr (kNext) nx = mfma32<F16>(a[i], q[i][0], nx);
+      } else if constexpr (kNow) {
+        constexpr int j = i - NS;
+        oacc[j % DB] = mfma32<F16>(vt[j], pk[j / DB], oacc[j % DB]);
+      }
+      if constexpr (kNow)
+        static_for<NG>([&](auto gc) SK_INLINE {
+          constexpr int g = decltype(gc)::value, f = g * FL / (NG - 1);
+          if constexpr (f == i) {
+            y[2 * g] = fmaf(sc[2 * g], mul, off);
+            y[2 * g + 1] = fmaf(sc[2 * g + 1], mul, off);
+          }
+          if constexpr (f + 1 == i) {
+            e[2 * g] = fast_exp2(y[2 * g]);
+            e[2 * g + 1] = fast_exp2(y[2 * g + 1]);
+          }
+          if constexpr (f + 2 == i) {
+            ps += e[2 * g] + e[2 * g + 1];
+            pk[g >> 2][g & 3] = pack2<F16>(e[2 * g], e[2 * g + 1]);
+            asm volatile("" : "+v"(ps));
+          }
+        });
+      // K in the first half of a tile's parts, V in the second.
+      if constexpr (h < NH / 2)
+        static_for<KST>([&](auto st) SK_INLINE {
+          if constexpr (decltype(st)::value * NM / KST == i)
+            widen_k(kb, std::integral_constant<int, h * KST + decltype(st)::value>{});
+        });
+      else
+        static_for<VST>([&](auto st) SK_INLINE {
+          if constexpr (decltype(st)::value * NM / VST == i)
+            widen_v(vb, std::integral_constant<int, (h - NH / 2) * VST + decltype(st)::value>{});
+        });
+      // The maximum of the new scores, from two slots behind their last MFMA.
+      if constexpr (kNext && i >= NS)
+        static_for<NG>([&](auto uc) SK_INLINE {
+          constexpr int u = decltype(uc)::value, at = NS + 2 + u * (NO - 2) / NG;
+          if constexpr (at == i) {
+            mx = fmaxf(mx, fmaxf(nx[2 * u], nx[2 * u + 1]));
+            asm volatile("" : "+v"(mx));
+          }
+        });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    if constexpr (kNow) ref.l += ps * to_l;
+  };
+
+  if (n_tiles > 0) {
+    constexpr int KB = BN * KSTR, VB = DP * VSTR;  // fp16 per buffer
+    // Pages of tiles 0 .. 3, then K(0), V(0), scales 0 and 1, K(1).
+    int pg0 = load_page(0), pg1 = load_page(1), pg2 = load_page(2), pg3 = load_page(3);
+    pg0 = settled_page(pg0), pg1 = settled_page(pg1), pg2 = settled_page(pg2), pg3 = settled_page(pg3);
+    load_k(0, pg0);
+    load_v(0, pg0);
+    const float sv0 = load_scale(0, pg0);
+    float sv = load_scale(1, pg1);
+    qmul = q8_query<KS, 1>(
+        p, b, hkv, r, sp.ql, [&](int s) SK_INLINE { return 16 * s + 8 * hi2; },
+        [](float x) SK_INLINE { return xhalf_max(x); }, q);
+    static_for<8>([&](auto st) SK_INLINE { widen_k(0, st); });
+    load_k(1, pg1);
+    static_for<4>([&](auto st) SK_INLINE { widen_v(0, st); });
+    load_v(1, pg1);
+    static_for<8>([&](auto st) SK_INLINE { widen_k(KB, st); });
+    load_k(2, pg2);
+    __syncthreads();
+    f32x16 sa = {}, sb;
+    float mx = kNegInf;
+    settle_scales(sv0, pg0);
+    if (w_tiles > 0) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) sa = mfma32<F16>(lds_read_b128(kfrom + 16 * s), q[s][0], sa);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sa[i]);
+      settle(k_lo, std::integral_constant<int, 0>{}, sa, mx);
+    }
+    // At tile t: k0, k1, k2: K buffers of t, t + 1 and of t + 2, being written; v0, v1:
+    // V's of t and t + 1, being written; sv: scales of t + 1, pg1 .. pg3: pages of t +
+    // 1 .. t + 3.
+    int k0 = 0, k1 = KB, k2 = 2 * KB, v0 = 0, v1 = VB;
+    auto tile = [&](int it, auto now, auto next) SK_INLINE {
+      constexpr bool kNow = decltype(now)::value;
+      const int n0 = k_lo + it * BN;
+      const int pg4 = load_page(it + 4);
+      const float sv2 = load_scale(it + 2, pg2);
+      static_for<NH>([&](auto part) SK_INLINE {
+        constexpr int h = decltype(part)::value;
+        if constexpr (h + 1 < NH) {
+          // The next part lies in this tile.
+          if constexpr (h % 2 == 0)
+            body(part, now, now, k0, v0, k2, v1, sa, sb, mx);
+          else
+            body(part, now, now, k0, v0, k2, v1, sb, sa, mx);
+          if constexpr (kNow) {
+            std::integral_constant<int, h + 1> after;
+            if constexpr (h % 2 == 0)
+              settle(n0, after, sb, mx);
+            else
+              settle(n0, after, sa, mx);
+          }
+        } else {
+          static_assert(NH % 2 == 0, "a tile starts with its scores in sa");
+          body(part, now, next, k1, v0, k2, v1, sb, sa, mx);
+          settle_scales(sv, pg1);
+          if constexpr (decltype(next)::value)
+            settle(n0 + BN, std::integral_constant<int, 0>{}, sa, mx);
+        }
+        if constexpr (h == NH / 2 - 1) load_k(it + 3, pg3);
+        if constexpr (h == NH - 1) load_v(it + 2, pg2);
+      });
+      sv = sv2;
+      pg1 = pg2, pg2 = pg3, pg3 = settled_page(pg4);
+      const int kx = k0;
+      k0 = k1, k1 = k2, k2 = kx;
+      const int vx = v0;
+      v0 = v1, v1 = vx;
+      __syncthreads();
+    };
+    // Tiles with another behind them, the wave's last one, and those that only other
+    // waves see (past the last tile nothing is loaded; zeros are widened).
+    int it = 0;
+    for (; it + 1 < w_tiles; ++it) tile(it, std::true_type{}, std::true_type{});
+    if (it < w_tiles) tile(it++, std::true_type{}, std::false_type{});
+    for (; it < n_tiles; ++it) tile(it, std::false_type{}, std::false_type{});
+  }
+
+  const float l = xhalf_sum(ref.l);
+  if (r >= p.rows) return;
+  const bool live = t < sp.ql;
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // (NaN stays NaN)
+  const float f = !live ? 0.f : ref.m2 == kNegInf ? inv : fast_exp2(ref.m2 - ref.m) * inv;
+  const int64_t row = (((int64_t)b * p.Hkv + hkv) * p.rows + r) * p.num_splits + split;
+  const int64_t at = (int64_t)b * p.o_sb + (int64_t)(hkv * p.group + r - t * p.group) * p.o_sh + (int64_t)t * p.o_ss;
+#pragma unroll
+  for (int i = 0; i < DB; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int d = 32 * i + 8 * j + 4 * hi2;
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = live ? oacc[i][4 * j + e] * f : 0.f;
+      if (p.num_splits > 1)
+        *reinterpret_cast<f32x4*>(p.part_o + row * DP + d) = f32x4{x[0], x[1], x[2], x[3]};
+      else if (d < p.D)
+        store_o4(p.o, p.dtype, at + d, x);
+    }
+  if (p.num_splits > 1 && hi2 == 0)
+    p.part_lse[row] = !live || l == 0.f ? kNegInf : ref.m == kNegInf ? l : ref.m + __log2f(l);
 }
 
 // Merge the splits of a row (query token, head), one wave a row: weights 2^(lse -
@@ -573,12 +1046,35 @@ static int q8_cols(int dtype, int D, int rows) {
   return want < most ? want : most;
 }
 
-int q8_rows_per_block(int dtype, int D, int rows) { return 16 * q8_cols(dtype, D, rows); }
+// Whether the kernel of many rows runs (16-bit queries): from 65 rows of a KV head
+// on.  8 KV heads of D = 128, each with its best split count, first kernel and this
+// one: 16 x 8,000 keys 64 and 93 us at 32 rows, 96 and 110 at 64, 144 and 123 at 96,
+// 291 and 186 at 256; 1 x 16,000 keys 25 and 27, 29 and 29, 35 and 31, 50 and 42.
+static bool q8_big(int dtype, int D, int rows) {
+  return dtype != SK_F32 && D <= 128 && rows > 64;
+}
+
+int q8_rows_per_block(int dtype, int D, int rows) {
+  return q8_big(dtype, D, rows) ? kQ8BigRows : 16 * q8_cols(dtype, D, rows);
+}
 
 int q8_splits(int dtype, int B, int Hkv, int rows, int keys, int D) {
   const int per = q8_rows_per_block(dtype, D, rows);
   const int64_t units = (int64_t)B * Hkv * ((rows + per - 1) / per);
   if (units <= 0) return 1;
+  if (q8_big(dtype, D, rows)) {
+    // Rounds of the 256 CUs (one workgroup each) times a piece's tiles and the fixed
+    // cost of a workgroup and of a row's partials, in tiles.
+    const int tiles = (keys * (D <= 64 ? 64 : 128) + 8191) / 8192;
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= 64 && (s == 1 || 2 * s <= tiles); ++s) {
+      const double rounds = (double)((units * s + 255) / 256);
+      const double cost = rounds * ((double)((tiles + s - 1) / s) + 6) + (s > 1 ? 4 + units * s / 64.0 : 0);
+      if (cost < least) least = cost, best = s;
+    }
+    return best;
+  }
   int64_t s = 1024 / units;
   const int64_t most = keys / 256;
   if (s > most) s = most;
@@ -606,8 +1102,27 @@ static hipError_t launch_dp(const Q8AttnParams& p, hipStream_t s) {
   return hipErrorInvalidValue;
 }
 
+template <class C, int DP>
+static hipError_t launch_big(const Q8AttnParams& p, hipStream_t s) {
+  using L = Q8Big<DP>;
+  const dim3 block(kQ8BigWaves * 64);
+  const dim3 grid((unsigned)((int64_t)p.B * p.Hkv * p.num_splits * p.row_blocks));
+  if (!p.table) {
+    hipLaunchKernelGGL((q8_big_kernel<C, DP, false, 1>), grid, block, 0, s, p);
+    return hipGetLastError();
+  }
+  if (p.page_size % L::BN != 0)
+    hipLaunchKernelGGL((q8_big_kernel<C, DP, true, L::NH>), grid, block, 0, s, p);
+  else
+    hipLaunchKernelGGL((q8_big_kernel<C, DP, true, 1>), grid, block, 0, s, p);
+  return hipGetLastError();
+}
+
 template <class C, int TERMS>
 static hipError_t launch_ct(const Q8AttnParams& p, hipStream_t s) {
+  if (q8_big(p.dtype, p.D, p.rows)) {
+    return p.D <= 64 ? launch_big<C, 64>(p, s) : launch_big<C, 128>(p, s);
+  }
   if (p.D <= 64) return launch_dp<C, TERMS, 64>(p, s);
   if (p.D <= 128) return launch_dp<C, TERMS, 128>(p, s);
   return launch_dp<C, TERMS, 256>(p, s);

@@ -243,6 +243,43 @@ def test_queries(device, code, dtype, sq):
 
 
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [16, 64, 80, 96, 128, 256])
+def test_many_rows(device, code, dtype, d):
+    """Chunks of more rows than a decode's: ragged, paged with the smallest pages and
+    contiguous, split and whole, rotated, and pages outside the pool."""
+    def change(table):
+        table[0, 1], table[0, 3] = -1, 10 ** 6
+
+    _attend(DTYPES[dtype], code, 4, 2, 40, d, 32, 32, [40, 200, 39, 1, 0, 260], [40, 37, 39, 5, 1, 40],
+            table_change=change)
+    _attend(DTYPES[dtype], code, 4, 2, 70, d, 64, 0, [300, 70, 7], [70, 69, 7], splits=3)
+    _attend(DTYPES[dtype], code, 2, 2, 129, d, 128, 128, [140, 257], causal=False)
+    _attend(DTYPES[dtype], code, 8, 1, 20, d, 32, 64, [150, 77], rope=True)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("sq", [1, 5, 40])
+def test_uneven_scales(device, code, sq):
+    """V scales that differ by far more than fp16 holds, zeros among them: what is small
+    next to the rest may vanish, the sum of the weights may not."""
+    b, hq, hkv, n, d = 2, 4, 2, 320, 64
+    kc, ks = _q8.make_cache(b, hkv, n, d, 32, code, seed=1)
+    vc, vs = _q8.make_cache(b, hkv, n, d, 32, code, seed=2)
+    size = torch.tensor([1.0, 1e-12, 0.0, 1e6, 1e-30, 1.0, 1e-38, 3.0, 0.0, 1e-4])
+    for order in (torch.arange(10), torch.arange(9, -1, -1)):
+        v2, k2 = vs * size[order], ks.clone()
+        k2[:, :, 4] = 0
+        q = _q8.randn(b, hq, sq, d, seed=3).bfloat16()
+        for splits in (1, 3):
+            got = attention_q8(q.cuda(), kc.cuda(), vc.cuda(), k2.cuda(), v2.cuda(), True,
+                               num_splits=splits)
+            want, tol = _q8.attention64(q, kc, vc, k2, v2, 32, [n] * b, [sq] * b, None, True, d ** -0.5,
+                                        splits)
+            _q8.check_within(got, want, tol)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
 @pytest.mark.parametrize("dtype,d", [("bf16", 128), ("fp16", 256), ("fp32", 64), ("bf16", 96)])
 def test_splits(device, code, dtype, d):
     """Explicit split counts: pieces without a key, single keys, more pieces than tiles."""
