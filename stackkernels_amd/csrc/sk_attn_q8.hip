@@ -797,10 +797,11 @@ __global__ void __launch_bounds__(kQ8BigWaves * 64) q8_big_kernel(Q8AttnParams p
   constexpr int NO = 2 * DB;    // output MFMAs
   constexpr int NM = NS + NO;
   constexpr int NG = 8;         // pairs of scores a lane holds
-  constexpr int KLEAD = 4, OLEAD = 6;  // MFMAs an operand is read ahead of its own
+  // MFMAs an operand is read ahead of its own.
+  constexpr int KLEAD = 4, OLEAD = NS < 6 ? NS : 6;
   constexpr int FL = NS + DB - 4;  // first slot of the last pair
   constexpr int KST = 16 / NH, VST = 8 / NH;  // widening steps of a body that has some
-  static_assert(FL > 0 && NM >= KST && NM >= VST, "slots");
+  static_assert(FL > 0 && NM >= KST && NM >= VST && KLEAD <= NS && OLEAD <= NS, "slots");
 
   const uint16_t* const kfrom = &ksm[0][c32 * KSTR + 8 * hi2];
   const uint16_t* const vfrom = &vsm[0][c32 * VSTR + 8 * (hi2 ^ (c32 / 16))];
