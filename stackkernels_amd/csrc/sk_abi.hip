@@ -1275,8 +1275,9 @@ int sk_attn_q8(const sk_q8_shape* shape, const void* q, const void* k_cache, con
   p.dpad = sk::q8_dpad(D);
   const int per = sk::q8_rows_per_block(dtype, D, p.rows);
   p.row_blocks = (p.rows + per - 1) / per;
-  if ((int64_t)B * Hkv * num_splits * p.row_blocks * 256 > 0xffffffffLL ||
-      (num_splits > 1 && (int64_t)B * Hq * Sq * 256 > 0xffffffffLL))
+  if ((int64_t)B * Hkv * num_splits * p.row_blocks * 512 > 0xffffffffLL ||
+      (num_splits > 1 && (int64_t)B * Hq * Sq * (num_splits > 16 ? 256 : 64) > 0xffffffffLL) ||
+      (int64_t)B * Hkv * num_splits * p.row_blocks > 0x7fffffffLL)
     return fail(SK_EINVAL, "grid too large: %d rows of %d queries, %d heads, %d splits", B, Sq, Hq,
                 num_splits);
   if (num_splits > 1) {

@@ -21,13 +21,23 @@
 //
 // Layout.  S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16 with 16 (query
 // token, head) rows of one KV head as the 16 columns, NC such blocks per wave.  A
-// wave takes 32 keys at a time straight from HBM into registers, no LDS:
-// * K: lane (key r, group g) loads the 16 bytes 64 j + 16 g of its key's row,
-//   two k-steps of eight consecutive head-dim columns; Q is laid out to match.
-// * V: lane (m, group g) loads columns [VB m, VB m + VB) (VB = DP / 16) of the
-//   eight keys whose probabilities group g holds; output block c is then the
-//   columns VB m + c, so the transposition V^T needs is a byte selection.
-// The four waves of a workgroup take tiles in turn and merge their sums in LDS.
+// wave takes 32 keys at a time through LDS of its own, which loads fill that pass no
+// register: up to two tiles are on their way while one is worked on, and no wave waits
+// for another before the end.  (Loads into registers instead: 655 -> 804 us for 64 x
+// 32,000 keys, D = 128, where the second wave of a SIMD did not fit.)
+// * Row 4 a + b of a 16-row operand block of K is key 4 b + a, so that group g's four
+//   results are keys 4 b + g and each load of V below covers whole rows.
+// * K: lane (key r, group g) brings the 16 bytes 64 j + 16 g of its key's row and
+//   reads them back itself, two k-steps of eight consecutive head-dim columns; Q is
+//   laid out to match.
+// * V: rows as they are; lane (m, group g) reads columns [VB m, VB m + VB) (VB = DP /
+//   16) of the eight keys whose probabilities group g holds; output block c is then
+//   the columns VB m + c, so the transposition V^T needs is a byte selection.
+// The waves of a workgroup take tiles in turn and merge their sums in LDS.
+//
+// What bounds it: long caches of many rows HBM (64 x 8 KV heads x 32,000 keys, D = 128:
+// 4.3 GB of codes in 655 us, 6.6 TB/s); few or short ones the chain of one tile, loads,
+// scores, maximum, probabilities, sums, about 1 us an iteration at D = 128.
 #include <type_traits>
 #include <utility>
 
@@ -128,8 +138,8 @@ __device__ __forceinline__ Q8Span q8_span(const Q8AttnParams& p, int b, int row0
   Q8Span s;
   s.len = p.seqlens ? min(max(__builtin_amdgcn_readfirstlane(p.seqlens[b]), 0), p.Sk) : p.Sk;
   s.ql = p.qlens ? min(max(__builtin_amdgcn_readfirstlane(p.qlens[b]), 0), p.Sq) : p.Sq;
-  const int t_first = row0 / p.group;
-  const int t_last = min((min(row0 + n_rows, p.rows) - 1) / p.group, s.ql - 1);
+  const int t_first = p.group_div.quot(row0);
+  const int t_last = min(p.group_div.quot(min(row0 + n_rows, p.rows) - 1), s.ql - 1);
   s.hi = p.causal ? min(s.len, s.len - s.ql + t_last + 1) : s.len;
   if (t_first >= s.ql) s.hi = 0;
   s.hi = max(s.hi, 0);
@@ -194,7 +204,7 @@ template <int KS, int TERMS, class Col, class Reduce>
 __device__ __forceinline__ float q8_query(const Q8AttnParams& p, int b, int hkv, int r, int ql,
                                           Col col, Reduce reduce, u32x4 (&out)[KS][TERMS]) {
   const int half = p.D >> 1;
-  const int t = r / p.group;
+  const int t = p.group_div.quot(r);
   const bool live = r < p.rows && t < ql;
   const int64_t at = live ? (int64_t)b * p.q_sb + (int64_t)(hkv * p.group + r - t * p.group) * p.q_sh +
                                 (int64_t)t * p.q_ss
@@ -243,28 +253,87 @@ __device__ __forceinline__ float q8_query(const Q8AttnParams& p, int b, int hkv,
   return __builtin_amdgcn_ldexpf(fabsf(p.scale_log2), ex);
 }
 
-constexpr int kQ8Waves = 4;
+// max / sum of a value across the lanes l and l ^ 16 (as xhalf_max: v_permlane16_swap
+// leaves a row of 16 lanes' own value in one result and the next row's in the other).
+__device__ __forceinline__ float xrow_max(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x),
+                                                  __builtin_bit_cast(uint32_t, x), false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float xrow_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x),
+                                                  __builtin_bit_cast(uint32_t, x), false, false);
+  return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
 
-// Column blocks whose queries are read from LDS each tile (the four waves share
-// them): with more than 32 head-dim-128 columns the sums alone take 128
-// registers, and the queries would take the second wave of a SIMD.
+// What a workgroup does: row block rb of piece split of the keys of (b, hkv), the
+// blocks that share keys next to one another on one XCD.
+struct Q8Item {
+  int rb, split, hkv, b;
+};
+__device__ __forceinline__ Q8Item q8_item(const Q8AttnParams& p) {
+  Q8Item w;
+  const int i = xcd_work_index(blockIdx.x, gridDim.x);
+  const int j = p.block_rows_div.quot(i);
+  w.rb = i - j * p.row_blocks;
+  const int k = p.split_div.quot(j);
+  w.split = j - k * p.num_splits;
+  w.b = p.hkv_div.quot(k);
+  w.hkv = k - w.b * p.Hkv;
+  return w;
+}
+
+// Until at most N loads are in flight.  (Also a fence to the compiler: what the wave
+// reads from LDS behind it stays behind it.)
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Waves of a workgroup: eight, sharing the queries in LDS, where the sums take half
+// the registers.
+template <int DP, int NC>
+constexpr int q8_waves() {
+  return NC * DP > 256 ? 8 : 4;
+}
+// Tiles in flight per wave: two, one where they take 16 KB each (two would leave a CU
+// four waves).
+template <int DP>
+constexpr int q8_stages() {
+  return DP > 128 ? 1 : 2;
+}
+
+// Column blocks whose queries are read from LDS each tile (the waves share them): with
+// more than 32 head-dim-128 columns the sums alone take 128 registers, and the queries
+// would take the second wave of a SIMD.
 template <int DP, int NC>
 constexpr bool q8_q_in_lds() {
   return NC * DP > 256;
 }
 
-template <class C, int TERMS, int DP, int NC, bool PAGED>
-__global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams p) {
+template <class C, int TERMS, int DP, int NC, int NW, bool PAGED>
+__global__ void __launch_bounds__(NW * 64, 2) q8_attn_kernel(Q8AttnParams p) {
   constexpr int KC = DP / 64;   // 16-byte chunks of a K row per lane
   constexpr int KS = DP / 32;   // k-steps of S^T
   constexpr int VB = DP / 16;   // bytes of a V row per lane = output blocks
   constexpr int VW = VB / 4;
-  constexpr int NW = kQ8Waves;
   constexpr bool kQLds = q8_q_in_lds<DP, NC>();
+  // Where registers allow: V is taken from LDS before the softmax, and a score's
+  // products run in two chains.
+  constexpr bool kEarly = NC * DP * TERMS <= 256;
+  constexpr int CH = NC == 1 ? 2 : 1;
 
+  constexpr int ST = q8_stages<DP>();
+  constexpr int KBYTES = 32 * DP;            // codes of K (and of V) of a tile
+  constexpr int LK = KBYTES / 1024;          // loads of them, 16 bytes a lane each
+  constexpr int STAGE = 2 * KBYTES;
+  constexpr int RING = NW * ST * STAGE;
+  constexpr int OUT = NW * 16 * (DP + 4) * 4;  // (the merge reuses the ring)
   __shared__ float red_m[NW][16 * NC];
   __shared__ float red_l[NW][16 * NC];
-  __shared__ __attribute__((aligned(16))) float red_o[NW][16][DP + 4];
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[RING > OUT ? RING : OUT];
+  __shared__ float meta[NW][ST][4];  // of a stage: k's and v's scale, a page
   __shared__ u32x4 qs[kQLds ? NC * KS * TERMS : 1][64];
   __shared__ float qmul_s[kQLds ? NC : 1][64];
 
@@ -274,94 +343,121 @@ __global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams 
   const int c16 = lane & 15;
   const int g = lane >> 4;
 
-  int item = xcd_work_index(blockIdx.x, gridDim.x);
-  const int rb = item % p.row_blocks;
-  item /= p.row_blocks;
-  const int split = item % p.num_splits;
-  item /= p.num_splits;
-  const int hkv = item % p.Hkv;
-  const int b = item / p.Hkv;
+  const Q8Item item = q8_item(p);
+  const int rb = item.rb, split = item.split, hkv = item.hkv, b = item.b;
 
   const int row0 = rb * 16 * NC;
   const Q8Span sp = q8_span(p, b, row0, 16 * NC);
-  const int kps = ((sp.hi + p.num_splits - 1) / p.num_splits + 31) / 32 * 32;
+  const int kps = (p.split_div.quot(sp.hi + p.num_splits - 1) + 31) / 32 * 32;
   const int k_lo = split * kps;
   const int k_hi = min(sp.hi, k_lo + kps);
 
   int lim[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c)
-    lim[c] = min(p.causal ? sp.len - sp.ql + (row0 + 16 * c + c16) / p.group + 1 : sp.len, k_hi);
+    lim[c] = min(p.causal ? sp.len - sp.ql + p.group_div.quot(row0 + 16 * c + c16) + 1 : sp.len, k_hi);
 
-  // This lane's loads within a tile: constant offsets from the tile's base.
-  const uint32_t k_off = (uint32_t)(c16 * (int)p.k.ss + 16 * g);
-  const uint32_t v_off = (uint32_t)(4 * g * (int)p.v.ss + VB * c16);
-  const bool v_in = VB * c16 < p.D;
+  // This lane's pieces of a tile.  K: load (kb, j) brings the 16 bytes the lane itself
+  // multiplies, which it finds at its own place again.  V: row by row.
+  const uint32_t k_off = (uint32_t)((4 * (c16 & 3) + (c16 >> 2)) * (int)p.k.ss + 16 * g);
+  constexpr int LPR = DP / 16;  // lanes per row of V
+  const uint32_t v_off = 16 * (lane % LPR) < p.D
+                             ? (uint32_t)(lane / LPR * (int)p.v.ss + 16 * (lane % LPR))
+                             : kBufferOob;
+  uint8_t* const my = ring + wave * ST * STAGE;
+  const uint32_t my_lds = __builtin_amdgcn_readfirstlane((int)lds_addr(my));
+  const uint32_t meta_lds = __builtin_amdgcn_readfirstlane((int)lds_addr(&meta[wave][0][0]));
+  const bool once = p.row_blocks == 1;  // read by this workgroup alone: past the caches
 
-  u32x4 kreg[2][KC];
-  uint32_t vreg[8][VW];
-  float ks_t = 0.f, vs_t = 0.f;  // scales of the tile in kreg / vreg
-  bool ok_t = false;
-  // The tile after it: its page (read a tile ahead) and where it lies.
-  int page_n = 0;
-  auto page_entry = [&](int n0) SK_INLINE {
-    return PAGED && n0 < k_hi ? p.table[(int64_t)b * p.max_pages + p.page_div.quot(n0)] : 0;
+  // Of tile it: its place in k, v and their scales, from its page.  With K of a tile
+  // come its two scales and the page of the tile that takes its stage next, 4 bytes
+  // each, so that the loop has no load whose wait could hold up another's.
+  struct Tile {
+    int64_t k, v;      // first elements
+    int64_t ks, vs;
+    int rows;          // visible keys, 0 past the last one and in a page outside the pool
   };
-  int64_t k_at = 0, v_at = 0;
-  int n_rows = 0;
-  // A buffer resource that ends with the tile's last visible row returns zeros for
-  // the rows past it (and for tiles whose page lies outside the pool).
-  auto load_k = [&](int n0, int page_raw) SK_INLINE {
-    int64_t unit = b;
-    int row = n0;
-    ok_t = true;
-    if constexpr (PAGED) {
-      const int page = __builtin_amdgcn_readfirstlane(page_raw);
-      ok_t = page >= 0 && page < p.num_pages;
-      unit = ok_t ? page : 0;
-      row = n0 - p.page_div.quot(n0) * p.page_size;
+  const int64_t unit0 = PAGED ? 0 : b;
+  const int64_t k_base = unit0 * p.k.sb + (int64_t)hkv * p.k.sh;
+  const int64_t v_base = unit0 * p.v.sb + (int64_t)hkv * p.v.sh;
+  const int64_t ks_base = unit0 * p.k.cb + (int64_t)hkv * p.k.ch;
+  const int64_t vs_base = unit0 * p.v.cb + (int64_t)hkv * p.v.ch;
+  const int* const table = PAGED ? p.table + (int64_t)b * p.max_pages : nullptr;
+  const int k_end = max(k_hi - 1, 0);
+  auto key_of = [&](int it) SK_INLINE { return k_lo + 32 * (wave + NW * it); };
+  auto page_at = [&](int it) SK_INLINE { return p.page_div.quot(min(key_of(it), k_end)); };
+  auto tile_of = [&](int it, int page) SK_INLINE {
+    const int n = key_of(it);
+    const bool ok = n < k_hi && (!PAGED || (page >= 0 && page < p.num_pages));
+    const uint32_t unit = PAGED && ok ? (uint32_t)page : 0u;
+    const uint32_t row = (uint32_t)(PAGED ? n - p.page_div.quot(n) * p.page_size : n);
+    const uint32_t blk = (uint32_t)p.block_div.quot((int)row);
+    Tile t;
+    t.k = k_base + (int64_t)((uint64_t)unit * (uint32_t)p.k.sb + (uint64_t)row * (uint32_t)p.k.ss);
+    t.v = v_base + (int64_t)((uint64_t)unit * (uint32_t)p.v.sb + (uint64_t)row * (uint32_t)p.v.ss);
+    t.ks = ks_base + (int64_t)((uint64_t)unit * (uint32_t)p.k.cb + (uint64_t)blk * (uint32_t)p.k.cs);
+    t.vs = vs_base + (int64_t)((uint64_t)unit * (uint32_t)p.v.cb + (uint64_t)blk * (uint32_t)p.v.cs);
+    t.rows = ok ? min(32, k_hi - n) : 0;
+    return t;
+  };
+  // Loads of a tile into stage st: every tile the same number, so the waits below
+  // count them.  A range that ends with the last visible row gives zeros for the rows
+  // past it.  reused: the wave's own reads of the stage come first.
+  constexpr int GK = LK + 2 + (PAGED ? 1 : 0), GV = LK;
+  auto load_k = [&](int it, const Tile& t, int st, auto reused) SK_INLINE {
+    const i32x4 r = uniform_words(
+        make_rsrc_words(p.k.codes + t.k, t.rows > 0 ? (t.rows - 1) * (int)p.k.ss + p.D : 0));
+    const i32x4 rk = uniform_words(make_rsrc_words(p.k.scales + t.ks, t.rows > 0 ? 4 : 0));
+    const i32x4 rv = uniform_words(make_rsrc_words(p.v.scales + t.vs, t.rows > 0 ? 4 : 0));
+    const uint32_t to = my_lds + st * STAGE;
+    if constexpr (decltype(reused)::value) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < LK; ++i) {
+      const int j = i % KC, kb = i / KC;
+      const uint32_t off = 64 * j + 16 * g < p.D ? k_off + (uint32_t)(16 * kb * (int)p.k.ss + 64 * j)
+                                                 : kBufferOob;
+      if (once)
+        buffer_load_lds_b128_nt(r, to + i * 1024, off);
+      else
+        buffer_load_lds_b128(r, to + i * 1024, off);
     }
-    n_rows = ok_t ? min(32, k_hi - n0) : 0;
-    k_at = unit * p.k.sb + (int64_t)hkv * p.k.sh + (int64_t)row * p.k.ss;
-    v_at = unit * p.v.sb + (int64_t)hkv * p.v.sh + (int64_t)row * p.v.ss;
-    const int blk = p.block_div.quot(row);
-    ks_t = ok_t ? p.k.scales[unit * p.k.cb + (int64_t)hkv * p.k.ch + (int64_t)blk * p.k.cs] : 0.f;
-    vs_t = ok_t ? p.v.scales[unit * p.v.cb + (int64_t)hkv * p.v.ch + (int64_t)blk * p.v.cs] : 0.f;
-    const buf_rsrc r =
-        make_rsrc(p.k.codes + k_at, n_rows > 0 ? (int)((n_rows - 1) * p.k.ss) + p.D : 0);
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int j = 0; j < KC; ++j)
-        kreg[kb][j] = buffer_load_b128(r, 64 * j + 16 * g < p.D
-                                              ? k_off + (uint32_t)(16 * kb * (int)p.k.ss + 64 * j)
-                                              : kBufferOob);
+    if (lane == 0) {
+      const uint32_t mt = meta_lds + st * 16;
+      buffer_load_lds_b32(rk, mt, 0);
+      buffer_load_lds_b32(rv, mt + 4, 0);
+      if constexpr (PAGED)
+        buffer_load_lds_b32(uniform_words(make_rsrc_words(table + page_at(it + ST), 4)), mt + 8, 0);
+    }
   };
-  auto load_v = [&]() SK_INLINE {
-    const buf_rsrc r =
-        make_rsrc(p.v.codes + v_at, n_rows > 0 ? (int)((n_rows - 1) * p.v.ss) + p.D : 0);
+  auto load_v = [&](const Tile& t, int st, auto reused) SK_INLINE {
+    const i32x4 r = uniform_words(
+        make_rsrc_words(p.v.codes + t.v, t.rows > 0 ? (t.rows - 1) * (int)p.v.ss + p.D : 0));
+    const uint32_t to = my_lds + st * STAGE + KBYTES;
+    if constexpr (decltype(reused)::value) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t off =
-          v_in ? v_off + (uint32_t)((e < 4 ? e : e + 12) * (int)p.v.ss) : kBufferOob;
-      if constexpr (VW == 1) {
-        vreg[e][0] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
-      } else if constexpr (VW == 2) {
-        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
-        vreg[e][0] = w[0], vreg[e][1] = w[1];
-      } else {
-        const u32x4 w = buffer_load_b128(r, off);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vreg[e][i] = w[i];
-      }
+    for (int i = 0; i < LK; ++i) {
+      const uint32_t off = v_off == kBufferOob ? v_off : v_off + (uint32_t)(i * (64 / LPR) * (int)p.v.ss);
+      if (once)
+        buffer_load_lds_b128_nt(r, to + i * 1024, off);
+      else
+        buffer_load_lds_b128(r, to + i * 1024, off);
     }
   };
 
-  int n0 = k_lo + 32 * wave;
-  if (n0 < k_hi) {
-    load_k(n0, page_entry(n0));
-    load_v();
-    page_n = page_entry(n0 + 32 * NW);
+  const int n_it = k_hi > k_lo + 32 * wave ? (k_hi - k_lo - 32 * wave + 32 * NW - 1) / (32 * NW) : 0;
+  int rows_t[ST] = {};  // of the tiles in the ring, oldest first
+  if (n_it > 0) {
+    int page[ST];
+#pragma unroll
+    for (int i = 0; i < ST; ++i)
+      page[i] = PAGED ? __builtin_amdgcn_readfirstlane(table[page_at(i)]) : 0;
+#pragma unroll
+    for (int i = 0; i < ST; ++i) {
+      const Tile t = tile_of(i, page[i]);
+      rows_t[i] = t.rows;
+      load_k(i, t, i, std::false_type{});
+      load_v(t, i, std::false_type{});
+    }
   }
 
   // Q^T operand: k-step s = 2 j + h of lane group g is head-dim columns 64 j +
@@ -370,7 +466,7 @@ __global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams 
   float qmul[NC];
   if (k_lo < k_hi) {
     auto col = [&](int s) SK_INLINE { return 64 * (s >> 1) + 16 * g + 8 * (s & 1); };
-    auto reduce = [](float x) SK_INLINE { return xhalf_max(fmaxf(x, __shfl_xor(x, 16))); };
+    auto reduce = [](float x) SK_INLINE { return xhalf_max(xrow_max(x)); };
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int r = row0 + 16 * c + c16;
@@ -398,20 +494,38 @@ __global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams 
 #pragma unroll
     for (int i = 0; i < VB; ++i) oacc[c][i] = f32x4{};
 
-  for (; n0 < k_hi; n0 += 32 * NW) {
-    const float ks = ks_t, vs = vs_t;
-    const bool ok = ok_t;
-    f32x4 sacc[NC][2];
+  int st = 0;
+  for (int it = 0; it < n_it; ++it) {
+    const int n0 = key_of(it);
+    const uint8_t* const kt = my + st * STAGE;
+    const uint8_t* const vt = kt + KBYTES;
+    // K(it) has landed: behind it at most V(it) and the other stages' loads.
+    wait_loads<GV + (ST - 1) * (GK + GV)>();
+    const float* const mt_at = &meta[wave][st][0];
+    const float ks = mt_at[0], vs = mt_at[1];
+    const int page = PAGED ? __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, mt_at[2])) : 0;
+    const bool ok = !PAGED || rows_t[0] > 0;
+    const Tile next = tile_of(it + ST, page);
 #pragma unroll
-    for (int c = 0; c < NC; ++c) sacc[c][0] = sacc[c][1] = f32x4{};
+    for (int i = 0; i + 1 < ST; ++i) rows_t[i] = rows_t[i + 1];
+    rows_t[ST - 1] = next.rows;
+    f32x4 sacc[NC][2], chain[NC][2][CH];
 #pragma unroll
-    for (int j = 0; j < KC; ++j)
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 2 * CH; ++i) chain[c][i & 1][i >> 1] = f32x4{};
+#pragma unroll
+    for (int j = 0; j < KC; ++j) {
+      u32x4 raw[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+        raw[kb] = *reinterpret_cast<const u32x4*>(kt + (kb * KC + j) * 1024 + lane * 16);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         u32x4 a[2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-          const uint32_t w0 = kreg[kb][j][2 * h], w1 = kreg[kb][j][2 * h + 1];
+          const uint32_t w0 = raw[kb][2 * h], w1 = raw[kb][2 * h + 1];
           a[kb] = u32x4{widen2<C, 0>(w0), widen2<C, 1>(w0), widen2<C, 0>(w1), widen2<C, 1>(w1)};
         }
 #pragma unroll
@@ -424,14 +538,39 @@ __global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams 
             else
               q = qreg[c][2 * j + h][u];
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) sacc[c][kb] = mfma16<F16>(a[kb], q, sacc[c][kb]);
+            for (int kb = 0; kb < 2; ++kb)
+              chain[c][kb][h % CH] = mfma16<F16>(a[kb], q, chain[c][kb][h % CH]);
           }
       }
-    const int n1 = n0 + 32 * NW;
-    if (n1 < k_hi) {
-      load_k(n1, page_n);
-      page_n = page_entry(n1 + 32 * NW);
     }
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+        sacc[c][kb] = CH == 1 ? chain[c][kb][0] : chain[c][kb][0] + chain[c][kb][CH - 1];
+    load_k(it + ST, next, st, std::true_type{});
+
+    uint32_t vreg[8][VW];
+    auto read_v = [&]() SK_INLINE {
+      // V(it) has landed: behind it the other stages' loads and K(it + ST).
+      wait_loads<(ST - 1) * (GK + GV) + GK>();
+  #pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint8_t* const at = vt + (4 * e + g) * DP + VB * c16;
+        if constexpr (VW == 1) {
+          vreg[e][0] = *reinterpret_cast<const uint32_t*>(at);
+        } else if constexpr (VW == 2) {
+          const u32x2 w = *reinterpret_cast<const u32x2*>(at);
+          vreg[e][0] = w[0], vreg[e][1] = w[1];
+        } else {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(at);
+  #pragma unroll
+          for (int i = 0; i < 4; ++i) vreg[e][i] = w[i];
+        }
+      }
+      load_v(next, st, std::true_type{});
+    };
+    if constexpr (kEarly) read_v();
 
     const bool masked = !ok || n0 + 32 > k_hi || n0 + 32 > sp.full;
     const float lv = __builtin_amdgcn_logf(vs);  // log2
@@ -446,12 +585,11 @@ __global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams 
         const int end = ok ? lim[c] : 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (n0 + 16 * (i >> 2) + 4 * g + (i & 3) >= end) e[i] = kNegInf;
+          if (n0 + 4 * i + g >= end) e[i] = kNegInf;
       }
       float mt = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])),
                        fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
-      mt = fmaxf(mt, __shfl_xor(mt, 16));
-      mt = xhalf_max(mt) * mul;
+      mt = xhalf_max(xrow_max(mt)) * mul;
       float ao;
       if (ref[c].raise(mt, mt + lv, ao)) {
 #pragma unroll
@@ -474,6 +612,7 @@ __global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams 
 #pragma unroll
       for (int i = 0; i < 4; ++i) split2<TERMS>(e[2 * i], e[2 * i + 1], pk[c][i]);
     }
+    if constexpr (!kEarly) read_v();
     auto product = [&](int w, auto hc) SK_INLINE {
       constexpr int H = decltype(hc)::value;
       u32x4 a0, a1;
@@ -498,15 +637,16 @@ __global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams 
       product(w, std::integral_constant<int, 0>{});
       product(w, std::integral_constant<int, 1>{});
     }
-    if (n1 < k_hi) load_v();
+    st = st + 1 == ST ? 0 : st + 1;
   }
+  wait_loads<0>();  // the loads past the last tile write zeros to the ring
 
+  float(*const red_o)[DP + 4] = reinterpret_cast<float(*)[DP + 4]>(ring);
   // Merge the four waves' sums: a row's common maximum M, then O scaled by 2^(m2 -
   // M) and l by 2^(m - M), added in wave order.
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    float l = ref[c].l + __shfl_xor(ref[c].l, 16);
-    l = xhalf_sum(l);
+    const float l = xhalf_sum(xrow_sum(ref[c].l));
     if (g == 0) {
       red_m[wave][16 * c + c16] = ref[c].m;
       red_l[wave][16 * c + c16] = l;
@@ -523,11 +663,11 @@ __global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams 
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int i = 0; i < VB; i += 4)
-        *reinterpret_cast<f32x4*>(&red_o[wave][c16][VB * (4 * g + r) + i]) =
+        *reinterpret_cast<f32x4*>(&red_o[wave * 16 + c16][VB * (4 * g + r) + i]) =
             f32x4{oacc[c][i][r], oacc[c][i + 1][r], oacc[c][i + 2][r], oacc[c][i + 3][r]} * f;
     __syncthreads();
     // 16 threads per row, DP / 16 columns each.
-    {
+    if (tid < 256) {
       const int rr = tid >> 4;
       const int d0 = (tid & 15) * VB;
       const int r = row0 + 16 * c + rr;
@@ -537,7 +677,7 @@ __global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams 
 #pragma unroll
       for (int w = 0; w < NW; ++w)
         lrow += red_l[w][16 * c + rr] * (mrow == kNegInf ? 1.f : fast_exp2(red_m[w][16 * c + rr] - mrow));
-      const int t = r / p.group;
+      const int t = p.group_div.quot(r);
       const bool live = r < p.rows && t < sp.ql;
       const float inv = lrow == 0.f ? 0.f : 1.f / lrow;  // (NaN stays NaN)
       if (r < p.rows) {
@@ -546,9 +686,9 @@ __global__ void __launch_bounds__(kQ8Waves * 64, 2) q8_attn_kernel(Q8AttnParams 
                            (int64_t)t * p.o_ss + d0;
 #pragma unroll
         for (int i = 0; i < VB; i += 4) {
-          f32x4 s = *reinterpret_cast<const f32x4*>(&red_o[0][rr][d0 + i]);
+          f32x4 s = *reinterpret_cast<const f32x4*>(&red_o[rr][d0 + i]);
 #pragma unroll
-          for (int w = 1; w < NW; ++w) s += *reinterpret_cast<const f32x4*>(&red_o[w][rr][d0 + i]);
+          for (int w = 1; w < NW; ++w) s += *reinterpret_cast<const f32x4*>(&red_o[w * 16 + rr][d0 + i]);
           float x[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[e] = live ? s[e] * inv : 0.f;
@@ -619,31 +759,27 @@ __global__ void __launch_bounds__(kQ8BigWaves * 64) q8_big_kernel(Q8AttnParams p
   const int c32 = lane & 31;
   const int hi2 = lane >> 5;
 
-  int item = xcd_work_index(blockIdx.x, gridDim.x);
-  const int rb = p.row_blocks - 1 - item % p.row_blocks;  // (causal: longest first)
-  item /= p.row_blocks;
-  const int split = item % p.num_splits;
-  item /= p.num_splits;
-  const int hkv = item % p.Hkv;
-  const int b = item / p.Hkv;
+  const Q8Item item = q8_item(p);
+  const int rb = p.row_blocks - 1 - item.rb;  // (causal: longest first)
+  const int split = item.split, hkv = item.hkv, b = item.b;
 
   const int row0 = rb * kQ8BigRows;
   const Q8Span sp = q8_span(p, b, row0, kQ8BigRows);
-  const int kps = ((sp.hi + p.num_splits - 1) / p.num_splits + BN - 1) / BN * BN;
+  const int kps = (p.split_div.quot(sp.hi + p.num_splits - 1) + BN - 1) / BN * BN;
   const int k_lo = split * kps;
   const int k_hi = min(sp.hi, k_lo + kps);
   const int n_tiles = k_hi > k_lo ? (k_hi - k_lo + BN - 1) / BN : 0;
   const int r = row0 + 32 * wave + c32;
-  const int t = r / p.group;
+  const int t = p.group_div.quot(r);
   const int lim = min(p.causal ? sp.len - sp.ql + t + 1 : sp.len, k_hi);
   // Tiles this wave's rows see, and keys that all of them see.
   const int w0 = row0 + 32 * wave;
   int w_tiles = 0, w_full = sp.len;
-  if (w0 < p.rows && w0 / p.group < sp.ql) {
-    const int last = min((min(w0 + 32, p.rows) - 1) / p.group, sp.ql - 1);
+  if (w0 < p.rows && p.group_div.quot(w0) < sp.ql) {
+    const int last = min(p.group_div.quot(min(w0 + 32, p.rows) - 1), sp.ql - 1);
     const int w_hi = p.causal ? min(sp.len - sp.ql + last + 1, k_hi) : k_hi;
     w_tiles = w_hi > k_lo ? (w_hi - k_lo + BN - 1) / BN : 0;
-    if (p.causal) w_full = sp.len - sp.ql + w0 / p.group + 1;
+    if (p.causal) w_full = sp.len - sp.ql + p.group_div.quot(w0) + 1;
   }
 
   // Where the codes of this KV head start (contiguous caches: of this row's too).
@@ -983,22 +1119,32 @@ __global__ void __launch_bounds__(kQ8BigWaves * 64) q8_big_kernel(Q8AttnParams p
     p.part_lse[row] = !live || l == 0.f ? kNegInf : ref.m == kNegInf ? l : ref.m + __log2f(l);
 }
 
-// Merge the splits of a row (query token, head), one wave a row: weights 2^(lse -
-// max) of the splits that saw a key, sums over lanes of 16 bytes of columns and, up
-// to 128 columns, over groups of lanes that take splits in turn.
-template <int DP>
+// Merge the splits of a row (query token, head): weights 2^(lse - max) of the splits
+// that saw a key, sums over lanes of 16 bytes of columns.  WPR waves take a row, DP /
+// 4 lanes a split; the first eight partials of each lane are on their way while the
+// weights are made.  Few splits: one wave a row; from 17 on: four.
+template <int DP, int WPR>
 __global__ void __launch_bounds__(256) q8_combine_kernel(Q8AttnParams p) {
-  constexpr int LPG = DP / 4;    // lanes per split
-  constexpr int G = 64 / LPG;    // splits at a time
+  constexpr int LPG = DP / 4;            // lanes per split
+  constexpr int G = 64 / LPG * WPR;      // splits at a time
+  constexpr int PRE = 8;
   __shared__ float w[4][kQ8MaxSplits];
+  __shared__ f32x4 part[WPR > 1 ? 4 : 1][LPG];
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
-  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
-  const int64_t bh = row / p.rows;
-  if (bh >= (int64_t)p.B * p.Hkv) return;
+  const int row = blockIdx.x * (4 / WPR) + (WPR > 1 ? 0 : wave);  // (below 2^31: host check)
+  const int bh = p.rows_div.quot(row);
+  if (bh >= p.B * p.Hkv) return;
   const int ns = p.num_splits;
-  const float* lse = p.part_lse + row * ns;
-  const float* po = p.part_o + row * ns * DP + (lane % LPG) * 4;
+  const float* lse = p.part_lse + (int64_t)row * ns;
+  const float* po = p.part_o + (int64_t)row * ns * DP + (lane % LPG) * 4;
+  const int first = lane / LPG + (WPR > 1 ? wave * (64 / LPG) : 0);
+  f32x4 pre[PRE];
+#pragma unroll
+  for (int k = 0; k < PRE; ++k) {
+    const int s = first + k * G;
+    pre[k] = s < ns ? *reinterpret_cast<const f32x4*>(po + (int64_t)s * DP) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   float mx = kNegInf;
   for (int s = lane; s < ns; s += 64) mx = fmaxf(mx, lse[s]);
 #pragma unroll
@@ -1012,10 +1158,16 @@ __global__ void __launch_bounds__(256) q8_combine_kernel(Q8AttnParams p) {
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) den += __shfl_xor(den, o);
-  // (The wave's own LDS writes: ordered before its reads.)
+  // (Each wave reads the weights it wrote itself: in order.  A split that saw no key
+  // has written no sums: whatever stands there is left out, not multiplied by 0.)
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = lane / LPG; s < ns; s += G) {
+#pragma unroll
+  for (int k = 0; k < PRE; ++k) {
+    const int s = first + k * G;
+    const float x = s < ns ? w[wave][s] : 0.f;
+    if (x != 0.f) acc += x * pre[k];
+  }
+  for (int s = first + PRE * G; s < ns; s += G) {
     const float x = w[wave][s];
     if (x != 0.f) acc += x * *reinterpret_cast<const f32x4*>(po + (int64_t)s * DP);
   }
@@ -1023,26 +1175,42 @@ __global__ void __launch_bounds__(256) q8_combine_kernel(Q8AttnParams p) {
   for (int o = LPG; o < 64; o <<= 1)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], o);
+  if constexpr (WPR > 1) {
+    if (lane < LPG) part[wave][lane] = acc;
+    __syncthreads();
+    if (wave > 0) return;
+    if (lane < LPG) acc = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+  }
   const int d = (lane % LPG) * 4;
   if (lane >= LPG || d >= p.D) return;
   const float inv = den == 0.f ? 0.f : 1.f / den;
-  const int r = (int)(row - bh * p.rows);
-  const int hkv = (int)(bh % p.Hkv);
-  const int64_t b = bh / p.Hkv;
-  const int t = r / p.group;
+  const int r = row - bh * p.rows;
+  const int64_t b = p.hkv_div.quot(bh);
+  const int hkv = bh - (int)b * p.Hkv;
+  const int t = p.group_div.quot(r);
   const float x[4] = {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
   store_o4(p.o, p.dtype,
            b * p.o_sb + (int64_t)(hkv * p.group + r - t * p.group) * p.o_sh + (int64_t)t * p.o_ss + d, x);
 }
 
+template <int DP>
+static hipError_t launch_combine(const Q8AttnParams& p, hipStream_t s) {
+  const int64_t rows = (int64_t)p.B * p.Hkv * p.rows;
+  if (p.num_splits > 16)
+    hipLaunchKernelGGL((q8_combine_kernel<DP, 4>), dim3((unsigned)rows), dim3(256), 0, s, p);
+  else
+    hipLaunchKernelGGL((q8_combine_kernel<DP, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, p);
+  return hipGetLastError();
+}
+
 int q8_dpad(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
-// Column blocks of 16 rows that a workgroup takes: as many as leave two waves a SIMD
-// without spills.  At D = 128 two blocks against one and four: 64 MQA heads, 8 x
-// 131,072 keys 114, 144 and 358 us (four spill); 512 queries against 16,000 keys
-// 252, 443 and 744; 2 x 4,096 against 16,384 1.84, 2.67 and 6.48 ms.
+// Column blocks of 16 rows that a workgroup takes: as many as the registers of a lane
+// hold the sums of.  One block against two and four, each with its best split count:
+// 64 rows, D = 128, 8 x 100,000 keys of one KV head 129, 91 and 64 us; 64 rows, D = 64,
+// 64 x 8,000 keys 98, 66 and 40.  (With more, fp32 queries and D > 128 would spill.)
 static int q8_cols(int dtype, int D, int rows) {
-  const int most = D > 128 ? 1 : D > 64 || dtype == SK_F32 ? 2 : 4;
+  const int most = D > 128 ? 1 : dtype == SK_F32 ? 2 : 4;
   const int want = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   return want < most ? want : most;
 }
@@ -1076,19 +1244,34 @@ int q8_splits(int dtype, int B, int Hkv, int rows, int keys, int D) {
     }
     return best;
   }
-  int64_t s = 1024 / units;
-  const int64_t most = keys / 256;
-  if (s > most) s = most;
-  return (int)(s < 1 ? 1 : s > kQ8MaxSplits ? kQ8MaxSplits : s);
+  // Microseconds, from times of 34 shapes over 1 to 128 splits (the chosen count came
+  // within 13% of the best one's time in all of them): a CU gets through an iteration
+  // (32 keys a wave) of its workgroups in about `step` however many it holds (at D <= 64
+  // three quarters of it past the first); 1.5 + nc is a workgroup's own cost; a quarter of its time is lost at the end, where CUs finish
+  // unevenly; splits cost the second kernel and the partials' traffic.
+  const int nc = per / 16, dp = q8_dpad(D), waves = nc * dp > 256 ? 8 : 4;
+  const double step = (0.4 + 0.36 * dp / 64) * (1 + 0.3 * (nc - 1)) * (waves == 8 ? 1.4 : 1.0);
+  const int tiles = (keys + 31) / 32;
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= kQ8MaxSplits && (s == 1 || s <= tiles / 2); ++s) {
+    const double run = ((tiles + s - 1) / s + waves - 1) / waves * step;
+    const double held = (double)((units * s + 255) / 256);
+    const double cost = (dp > 64 ? held : 0.25 + 0.75 * held) * (run + 1.5 + nc) + 0.25 * run +
+                        (s > 1 ? 3 + (double)B * Hkv * rows * s * dp * 2.5e-6 : 0);
+    if (cost < 0.99 * least) least = cost, best = s;
+  }
+  return best;
 }
 
 template <class C, int TERMS, int DP, int NC>
 static hipError_t launch_nc(const Q8AttnParams& p, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)p.B * p.Hkv * p.num_splits * p.row_blocks));
+  constexpr int NW = q8_waves<DP, NC>();
   if (p.table)
-    hipLaunchKernelGGL((q8_attn_kernel<C, TERMS, DP, NC, true>), grid, dim3(kQ8Waves * 64), 0, s, p);
+    hipLaunchKernelGGL((q8_attn_kernel<C, TERMS, DP, NC, NW, true>), grid, dim3(NW * 64), 0, s, p);
   else
-    hipLaunchKernelGGL((q8_attn_kernel<C, TERMS, DP, NC, false>), grid, dim3(kQ8Waves * 64), 0, s, p);
+    hipLaunchKernelGGL((q8_attn_kernel<C, TERMS, DP, NC, NW, false>), grid, dim3(NW * 64), 0, s, p);
   return hipGetLastError();
 }
 
@@ -1098,7 +1281,7 @@ static hipError_t launch_dp(const Q8AttnParams& p, hipStream_t s) {
   if (nc == 1) return launch_nc<C, TERMS, DP, 1>(p, s);
   if constexpr (DP <= 128)
     if (nc == 2) return launch_nc<C, TERMS, DP, 2>(p, s);
-  if constexpr (DP <= 64 && TERMS == 1)
+  if constexpr (DP <= 128 && TERMS == 1)
     if (nc == 4) return launch_nc<C, TERMS, DP, 4>(p, s);
   return hipErrorInvalidValue;
 }
@@ -1129,20 +1312,19 @@ static hipError_t launch_ct(const Q8AttnParams& p, hipStream_t s) {
   return launch_dp<C, TERMS, 256>(p, s);
 }
 
-hipError_t launch_q8_attn(int code, const Q8AttnParams& p, hipStream_t s) {
+hipError_t launch_q8_attn(int code, const Q8AttnParams& p0, hipStream_t s) {
+  Q8AttnParams p = p0;
+  p.group_div = FastDiv(p.group);
+  p.rows_div = FastDiv(p.rows);
+  p.hkv_div = FastDiv(p.Hkv);
+  p.split_div = FastDiv(p.num_splits);
+  p.block_rows_div = FastDiv(p.row_blocks);
   const bool wide = p.dtype == SK_F32;
   const hipError_t e =
       code == kCodeI8 ? (wide ? launch_ct<I8, 2>(p, s) : launch_ct<I8, 1>(p, s))
                       : (wide ? launch_ct<E4M3, 2>(p, s) : launch_ct<E4M3, 1>(p, s));
   if (e != hipSuccess || p.num_splits == 1) return e;
-  const dim3 grid((unsigned)(((int64_t)p.B * p.Hkv * p.rows + 3) / 4));
-  if (p.dpad == 64)
-    hipLaunchKernelGGL(q8_combine_kernel<64>, grid, dim3(256), 0, s, p);
-  else if (p.dpad == 128)
-    hipLaunchKernelGGL(q8_combine_kernel<128>, grid, dim3(256), 0, s, p);
-  else
-    hipLaunchKernelGGL(q8_combine_kernel<256>, grid, dim3(256), 0, s, p);
-  return hipGetLastError();
+  return p.dpad == 64 ? launch_combine<64>(p, s) : p.dpad == 128 ? launch_combine<128>(p, s) : launch_combine<256>(p, s);
 }
 
 }  // namespace sk

@@ -99,6 +99,7 @@ struct Q8AttnParams {
   const int* table;      // null: contiguous
   int page_size, max_pages, num_pages;
   FastDiv block_div, page_div;
+  FastDiv group_div, rows_div, hkv_div, split_div, block_rows_div;  // (set by the launcher)
   RopeParams rope;
 };
 
