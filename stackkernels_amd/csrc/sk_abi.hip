@@ -1203,7 +1203,7 @@ int sk_kv_cache_update_q8(const sk_q8_shape* shape, const void* k, const void* v
   p.page_size = rows, p.max_pages = sh.max_pages, p.num_pages = sh.units;
   p.block = sh.block_size;
   p.blocks = (int)(((int64_t)T + p.block - 2) / p.block + 1);
-  if ((int64_t)B * p.blocks * Hkv * 2 * 256 > 0xffffffffLL)
+  if (((int64_t)B * p.blocks + 7) / 8 * 16 * Hkv * 256 > 0xffffffffLL)
     return fail(SK_EINVAL, "grid too large: %d rows of %d new tokens, %d heads", B, T, Hkv);
   const hipError_t e = sk::launch_q8_append(sh.dtype, sh.code, p, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(e, "sk_kv_cache_update_q8 launch");

@@ -1245,7 +1245,7 @@ int q8_splits(int dtype, int B, int Hkv, int rows, int keys, int D) {
     return best;
   }
   // Microseconds, from times of 34 shapes over 1 to 128 splits (the chosen count came
-  // within 13% of the best one's time in all of them): a CU gets through an iteration
+  // within 10% of the best one's time in all of them): a CU gets through an iteration
   // (32 keys a wave) of its workgroups in about `step` however many it holds (at D <= 64
   // three quarters of it past the first); 1.5 + nc is a workgroup's own cost; a quarter of its time is lost at the end, where CUs finish
   // unevenly; splits cost the second kernel and the partials' traffic.

@@ -13,8 +13,12 @@
 //
 // One workgroup owns a (batch row, block, KV head, k or v): amax, scale and codes
 // need no atomics and results do not depend on order.  Bound by the new tokens'
-// bytes (2 or 4 in, 1 out per element); the older codes of a block are read only
-// when its scale grows.
+// bytes (2 or 4 in, 1 out per element) and by the rotation's entries, 8 bytes per
+// element of K, from the caches; the older codes of a block are read only when its
+// scale grows.  8 x 2,048 tokens, 8 heads, D = 128, fp16, ragged lengths (59 MB, 11.4
+// us as a copy): 20.4 us, 15.4 unrotated (31.2 and 23.5 with each element of K read
+// twice and every element's infinity and NaN looked for one by one; 21.7 with a
+// block's heads on all XCDs).  One token: 5.3 us, a launch and two dependent loads.
 #include <type_traits>
 
 #include "sk_common.h"
@@ -40,11 +44,24 @@ __device__ __forceinline__ float needed_scale(float amax) {
 }
 
 // Four scaled values as four codes, nearest (ties to even), saturated.  NaN: code
-// 0 in int8 (which has none), NaN in e4m3.
-template <int CODE>
+// 0 in int8 (which has none), NaN in e4m3.  FINITE: none is infinite or NaN, and
+// none exceeds the largest code by more than its scale's rounding, so that nothing
+// needs saturating: in int8 the sum with 1.5 2^23 leaves the rounded number's low
+// byte in place.
+template <int CODE, bool FINITE>
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
   if constexpr (CODE == kCodeI8) {
-    const float x[4] = {a, b, c, d};
+    float x[4] = {a, b, c, d};
+    if constexpr (FINITE) {
+      uint32_t u[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        asm("" : "+v"(x[i]));  // (a rounded product, never fused into the sum)
+        u[i] = __builtin_bit_cast(uint32_t, x[i] + 12582912.f);
+      }
+      return __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[3], u[2], 0x0c0c0400u),
+                                   __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), 0x05040100u);
+    }
     uint32_t w = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -53,7 +70,9 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
     }
     return w;
   } else {
-    auto sat = [](float y) { return y == y ? fminf(fmaxf(y, -448.f), 448.f) : y; };
+    auto sat = [](float y) SK_INLINE {
+      return FINITE ? y : y == y ? fminf(fmaxf(y, -448.f), 448.f) : y;
+    };
     uint32_t w = __builtin_amdgcn_cvt_pk_fp8_f32(sat(a), sat(b), 0, false);
     return __builtin_amdgcn_cvt_pk_fp8_f32(sat(c), sat(d), w, true);
   }
@@ -90,123 +109,173 @@ __device__ __forceinline__ void load8(const void* base, int64_t at, float (&x)[8
   }
 }
 
-// Chunks of eight elements that a thread keeps in registers between the pass for
-// amax and the pass that writes codes; a block with more re-reads the rest.
-constexpr int kKeep = 8;
-
-template <class T, int CODE, int NT>
-__global__ void __launch_bounds__(NT) q8_append_kernel(Q8AppendParams p) {
-  __shared__ float red[NT / 64];
+// A thread takes pairs of eight columns, d .. d + 7 and D / 2 + d .. + 7 of a token:
+// what a rotation mixes, each element read once.  The first KEEP pairs of a thread
+// stay in registers between the pass for amax and the pass that writes codes; a
+// larger block re-reads the rest.  (Five waves a SIMD cost two spilled registers and
+// gain 3% over four.)
+template <class T, int CODE, int NT, int KEEP>
+__global__ void __launch_bounds__(NT, KEEP == 2 ? 5 : 3) q8_append_kernel(Q8AppendParams p) {
+  __shared__ float red[2][NT / 64];
   const int tid = threadIdx.x;
-  int item = blockIdx.x;
-  const int kv = item & 1;
-  item >>= 1;
-  const int h = item % p.Hkv;
-  item /= p.Hkv;
-  const int j = item % p.blocks;
-  const int b = item / p.blocks;
-  const int start = max(p.lens[b], 0);
-  const int n_new = p.news ? min(max(p.news[b], 0), p.T) : p.T;
+  // The 2 Hkv workgroups of a block follow one another on one XCD (workgroups go to
+  // the eight round robin), which then reads the rotation's entries once.
+  const int turn = blockIdx.x >> 3;
+  const int kv = turn & 1;
+  const int group = p.hkv_div.quot(turn >> 1);
+  const int h = (turn >> 1) - group * p.Hkv;
+  const int bj = group * 8 + (blockIdx.x & 7);
+  if (bj >= p.B * p.blocks) return;
+  const int b = p.blocks_div.quot(bj);
+  const int j = bj - b * p.blocks;
+  const int start = max(__builtin_amdgcn_readfirstlane(p.lens[b]), 0);
+  const int n_new = p.news ? min(max(__builtin_amdgcn_readfirstlane(p.news[b]), 0), p.T) : p.T;
   if (n_new == 0 || start >= p.cap) return;
   // Tokens [lo, lo + block) of the row; the new ones among them [a, z).
-  const int64_t lo = ((int64_t)start / p.block + j) * p.block;
-  const int64_t a = lo > start ? lo : start;
-  int64_t z = (int64_t)start + n_new;
-  z = z < p.cap ? z : p.cap;
-  z = z < lo + p.block ? z : lo + p.block;
-  if (a >= z) return;
-  int64_t unit = b, row = lo;
+  const int64_t lo64 = ((int64_t)p.block_div.quot(start) + j) * p.block;
+  const int64_t end = min((int64_t)start + n_new, (int64_t)p.cap);
+  if (lo64 >= end) return;
+  const int lo = (int)lo64;  // (below cap)
+  const int a = max(lo, start);
+  const int z = (int)min(end, lo64 + p.block);
+  int64_t unit = b;
+  int row = lo;
   if (p.table) {
-    const int page = p.table[(int64_t)b * p.max_pages + (int)(lo / p.page_size)];
+    const int at = p.page_div.quot(lo);
+    const int page = __builtin_amdgcn_readfirstlane(p.table[(int64_t)b * p.max_pages + at]);
     if (page < 0 || page >= p.num_pages) return;
     unit = page;
-    row = lo % p.page_size;
+    row = lo - at * p.page_size;
   }
   const Q8Cache& c = p.c[kv];
-  uint8_t* codes = c.codes + unit * c.sb + (int64_t)h * c.sh + row * c.ss;
-  float* scale = c.scales + unit * c.cb + (int64_t)h * c.ch + (row / p.block) * c.cs;
-  const int older = (int)(a - lo);
-  const int cpr = p.D / 8;  // chunks per token
-  const int n = (int)(z - a) * cpr;
-  const int t0 = (int)(a - start);
+  uint8_t* codes = c.codes + unit * c.sb + (int64_t)h * c.sh + (int64_t)row * c.ss;
+  float* scale = c.scales + unit * c.cb + (int64_t)h * c.ch + (int64_t)p.block_div.quot(row) * c.cs;
+  const int older = a - lo;
   const int half = p.D >> 1;
+  const int ppr = p.D >> 4;  // pairs per token
+  const int n = (z - a) * ppr;
+  const int t0 = a - start;
+  const float had = older > 0 ? *scale : 0.f;
+  const int64_t x0 = (int64_t)b * p.x_sb[kv] + (int64_t)h * p.x_sh[kv] + (int64_t)t0 * p.x_ss[kv];
+  const int64_t x_ss = p.x_ss[kv];
 
-  auto fetch = [&](int i, float (&x)[8]) SK_INLINE {
-    const int r = i / cpr;
-    const int d0 = (i - r * cpr) * 8;
-    const int64_t at = (int64_t)b * p.x_sb[kv] + (int64_t)h * p.x_sh[kv] + (int64_t)(t0 + r) * p.x_ss[kv];
-    load8<T>(p.x[kv], at + d0, x);
+  auto fetch = [&](int i, float (&x)[2][8]) SK_INLINE {
+    const int r = p.pairs_div.quot(i);
+    const int d0 = (i - r * ppr) * 8;
+    const int64_t at = x0 + r * x_ss + d0;
+    load8<T>(p.x[kv], at, x[0]);
+    load8<T>(p.x[kv], at + half, x[1]);
     if (kv == 0) {
       const int rr = rope_row(p.rope, b, t0 + r);
       if (rr >= 0) {
-        float y[8], cs[8], sn[8];
-        load8<T>(p.x[kv], at + (d0 < half ? d0 + half : d0 - half), y);
-        rope_coeffs<8>(p.rope, rr, d0, cs, sn);
+        float cs[2][8], sn[2][8];
+        rope_coeffs<8>(p.rope, rr, d0, cs[0], sn[0]);
+        rope_coeffs<8>(p.rope, rr, d0 + half, cs[1], sn[1]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = rope_mix(x[e], y[e], d0 < half, cs[e], sn[e]);
+        for (int e = 0; e < 8; ++e) {
+          const float u = x[0][e], v = x[1][e];
+          x[0][e] = rope_mix(u, v, true, cs[0][e], sn[0][e]);
+          x[1][e] = rope_mix(v, u, false, cs[1][e], sn[1][e]);
+        }
       }
     }
   };
-  float amax = 0.f;
-  auto widest = [&](const float (&x)[8]) SK_INLINE {
+  // amax: of the elements that are numbers.  zero becomes NaN at an infinity or NaN.
+  float amax = 0.f, zero = 0.f;
+  auto widest = [&](const float (&x)[2][8]) SK_INLINE {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float y = fabsf(x[e]);
-      amax = y < __builtin_inff() ? fmaxf(amax, y) : amax;
+      amax = fmaxf(fmaxf(amax, fabsf(x[0][e])), fabsf(x[1][e]));
+      zero = __builtin_fmaf(x[0][e], 0.f, zero);
+      zero = __builtin_fmaf(x[1][e], 0.f, zero);
     }
   };
-  float keep[kKeep][8];
+  float keep[KEEP][2][8];
 #pragma unroll
-  for (int i = 0; i < kKeep; ++i)
-    if (tid + i * NT < n) {
-      fetch(tid + i * NT, keep[i]);
-      widest(keep[i]);
-    }
-  for (int i = tid + kKeep * NT; i < n; i += NT) {
-    float x[8];
+  for (int i = 0; i < KEEP; ++i)
+    if (tid + i * NT < n) fetch(tid + i * NT, keep[i]);
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i)
+    if (tid + i * NT < n) widest(keep[i]);
+  for (int i = tid + KEEP * NT; i < n; i += NT) {
+    float x[2][8];
     fetch(i, x);
     widest(x);
   }
+  // Over the workgroup.
+  auto joined = [&](float x, float (&out)[NT / 64]) SK_INLINE {
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-  if constexpr (NT > 64) {
-    if ((tid & 63) == 0) red[tid >> 6] = amax;
-    __syncthreads();
+    for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
+    if constexpr (NT > 64) {
+      if ((tid & 63) == 0) out[tid >> 6] = x;
+      __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NT / 64; ++w) amax = fmaxf(amax, red[w]);
+      for (int w = 0; w < NT / 64; ++w) x = fmaxf(x, out[w]);
+    }
+    return x;
+  };
+  amax = joined(zero == 0.f ? amax : __builtin_inff(), red[0]);
+  const bool finite = amax < __builtin_inff();
+  if (!finite) {
+    // Some elements are not: the largest of those that are.
+    amax = 0.f;
+    auto widest_finite = [&](const float (&x)[2][8]) SK_INLINE {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float y = fabsf(x[e >> 3][e & 7]);
+        amax = y < __builtin_inff() ? fmaxf(amax, y) : amax;
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+      if (tid + i * NT < n) widest_finite(keep[i]);
+    for (int i = tid + KEEP * NT; i < n; i += NT) {
+      float x[2][8];
+      fetch(i, x);
+      widest_finite(x);
+    }
+    amax = joined(amax, red[1]);
   }
   const float need = needed_scale<CODE>(amax);
-  const float had = older > 0 ? *scale : 0.f;
   const float now = older > 0 && had > need ? had : need;
   const float inv = 1.f / now;
-  auto put = [&](int i, const float (&x)[8]) SK_INLINE {
-    const int r = i / cpr;
-    const int d0 = (i - r * cpr) * 8;
-    const u32x2 w = {
-        encode4<CODE>(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv),
-        encode4<CODE>(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv)};
-    *reinterpret_cast<u32x2*>(codes + (int64_t)(older + r) * c.ss + d0) = w;
-  };
+  auto put = [&](int i, const float (&x)[2][8], auto fin) SK_INLINE {
+    const int r = p.pairs_div.quot(i);
+    uint8_t* at = codes + (int64_t)(older + r) * c.ss + (i - r * ppr) * 8;
+    constexpr bool F = decltype(fin)::value;
 #pragma unroll
-  for (int i = 0; i < kKeep; ++i)
-    if (tid + i * NT < n) put(tid + i * NT, keep[i]);
-  for (int i = tid + kKeep * NT; i < n; i += NT) {
-    float x[8];
-    fetch(i, x);
-    put(i, x);
-  }
+    for (int q = 0; q < 2; ++q) {
+      const float (&v)[8] = x[q];
+      *reinterpret_cast<u32x2*>(at + q * half) =
+          u32x2{encode4<CODE, F>(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+                encode4<CODE, F>(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv)};
+    }
+  };
+  auto write = [&](auto fin) SK_INLINE {
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+      if (tid + i * NT < n) put(tid + i * NT, keep[i], fin);
+    for (int i = tid + KEEP * NT; i < n; i += NT) {
+      float x[2][8];
+      fetch(i, x);
+      put(i, x, fin);
+    }
+  };
+  if (finite)
+    write(std::true_type{});
+  else
+    write(std::false_type{});
   if (older > 0 && had < now) {
     const float f = had / now;
-    for (int i = tid; i < older * cpr; i += NT) {
-      const int r = i / cpr;
-      const int d0 = (i - r * cpr) * 8;
-      u32x2* at = reinterpret_cast<u32x2*>(codes + (int64_t)r * c.ss + d0);
+    for (int i = tid; i < older * 2 * ppr; i += NT) {
+      const int r = p.pairs_div.quot(i >> 1);
+      u32x2* at = reinterpret_cast<u32x2*>(codes + (int64_t)r * c.ss + (i - 2 * r * ppr) * 8);
       u32x2 w = *at;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         float x[4];
         decode4<CODE>(w[q], x);
-        w[q] = encode4<CODE>(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
+        w[q] = encode4<CODE, false>(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
       }
       *at = w;
     }
@@ -216,15 +285,24 @@ __global__ void __launch_bounds__(NT) q8_append_kernel(Q8AppendParams p) {
 }
 
 template <class T, int CODE>
-static hipError_t append_tc(const Q8AppendParams& p, hipStream_t s) {
-  const int64_t items = (int64_t)p.B * p.blocks * p.Hkv * 2;
-  if (items == 0) return hipSuccess;
-  // One wave where a block's new elements fit its registers twice over.
-  const int64_t elems = (int64_t)(p.T < p.block ? p.T : p.block) * p.D;
-  if (elems <= 64 * 8 * kKeep)
-    hipLaunchKernelGGL((q8_append_kernel<T, CODE, 64>), dim3((unsigned)items), dim3(64), 0, s, p);
+static hipError_t append_tc(const Q8AppendParams& p0, hipStream_t s) {
+  Q8AppendParams p = p0;
+  if ((int64_t)p.B * p.blocks * p.Hkv == 0) return hipSuccess;
+  p.block_div = FastDiv(p.block);
+  p.hkv_div = FastDiv(p.Hkv);
+  p.blocks_div = FastDiv(p.blocks);
+  p.pairs_div = FastDiv(p.D / 16);
+  if (p.table) p.page_div = FastDiv(p.page_size);
+  const int64_t pairs = (int64_t)(p.T < p.block ? p.T : p.block) * (p.D / 16);
+  const dim3 grid((unsigned)(((int64_t)p.B * p.blocks + 7) / 8 * 16 * p.Hkv));
+  // Two pairs a thread (of one wave, or of four), four in the largest blocks: one and
+  // four pairs a thread of as many as make up a block took 25.3 and 24.5 us above.
+  if (pairs <= 64 * 2)
+    hipLaunchKernelGGL((q8_append_kernel<T, CODE, 64, 2>), grid, dim3(64), 0, s, p);
+  else if (pairs <= 256 * 2)
+    hipLaunchKernelGGL((q8_append_kernel<T, CODE, 256, 2>), grid, dim3(256), 0, s, p);
   else
-    hipLaunchKernelGGL((q8_append_kernel<T, CODE, 256>), dim3((unsigned)items), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((q8_append_kernel<T, CODE, 256, 4>), grid, dim3(256), 0, s, p);
   return hipGetLastError();
 }
 

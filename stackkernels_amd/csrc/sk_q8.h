@@ -75,6 +75,7 @@ struct Q8AppendParams {
   int page_size, max_pages, num_pages;
   int block;
   int blocks;            // blocks a row's new tokens can touch
+  FastDiv block_div, hkv_div, blocks_div, pairs_div, page_div;  // (set by the launcher)
   RopeParams rope;       // keys only
 };
 
