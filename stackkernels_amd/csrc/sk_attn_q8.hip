@@ -176,12 +176,19 @@ struct Q8Ref {
   // by more than kRescaleLog2 (smaller excesses only make e larger than 1): ao is
   // then the factor of the row's sums.
   __device__ __forceinline__ bool raise(float mt, float mt2, float& ao) {
-    if (!__any(mt > m + kRescaleLog2 || mt2 > m2 + kRescaleLog2)) return false;
+    if (!__any(exceeded(mt, mt2))) return false;
+    ao = raised(mt, mt2);
+    return true;
+  }
+  __device__ __forceinline__ bool exceeded(float mt, float mt2) const {
+    return mt > m + kRescaleLog2 || mt2 > m2 + kRescaleLog2;
+  }
+  __device__ __forceinline__ float raised(float mt, float mt2) {
     const float m_new = fmaxf(m, mt), m2_new = fmaxf(m2, mt2);
     l *= m_new == kNegInf ? 1.f : fast_exp2(m - m_new);
-    ao = m2_new == kNegInf ? 1.f : fast_exp2(m2 - m2_new);
+    const float ao = m2_new == kNegInf ? 1.f : fast_exp2(m2 - m2_new);
     m = m_new, m2 = m2_new;
-    return true;
+    return ao;
   }
   // lv: log2 of the tile's V scale.  (A row that has seen no key has only -inf
   // scores, whose e is 0 for any finite offset.)
@@ -554,7 +561,7 @@ __global__ void __launch_bounds__(NW * 64, 2) q8_attn_kernel(Q8AttnParams p) {
     auto read_v = [&]() SK_INLINE {
       // V(it) has landed: behind it the other stages' loads and K(it + ST).
       wait_loads<(ST - 1) * (GK + GV) + GK>();
-  #pragma unroll
+#pragma unroll
       for (int e = 0; e < 8; ++e) {
         const uint8_t* const at = vt + (4 * e + g) * DP + VB * c16;
         if constexpr (VW == 1) {
@@ -564,7 +571,7 @@ __global__ void __launch_bounds__(NW * 64, 2) q8_attn_kernel(Q8AttnParams p) {
           vreg[e][0] = w[0], vreg[e][1] = w[1];
         } else {
           const u32x4 w = *reinterpret_cast<const u32x4*>(at);
-  #pragma unroll
+#pragma unroll
           for (int i = 0; i < 4; ++i) vreg[e][i] = w[i];
         }
       }
@@ -575,40 +582,54 @@ __global__ void __launch_bounds__(NW * 64, 2) q8_attn_kernel(Q8AttnParams p) {
     const bool masked = !ok || n0 + 32 > k_hi || n0 + 32 > sp.full;
     const float lv = __builtin_amdgcn_logf(vs);  // log2
     uint32_t pk[NC][4][TERMS];
+    // All blocks' maxima first and one test for all of them: their chains then run
+    // side by side.
+    float mul[NC], mt[NC];
+    bool above = false;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const float mul = fmaxf(ks * qmul[c], kMinFactor);
-      float e[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = sacc[c][i >> 2][i & 3];
+      mul[c] = fmaxf(ks * qmul[c], kMinFactor);
       if (masked) {
         const int end = ok ? lim[c] : 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (n0 + 4 * i + g >= end) e[i] = kNegInf;
+          if (n0 + 4 * i + g >= end) sacc[c][i >> 2][i & 3] = kNegInf;
       }
-      float mt = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])),
-                       fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
-      mt = xhalf_max(xrow_max(mt)) * mul;
-      float ao;
-      if (ref[c].raise(mt, mt + lv, ao)) {
+      const f32x4 &a = sacc[c][0], &b = sacc[c][1];
+      mt[c] = fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), fmaxf(fmaxf(b[0], b[1]), fmaxf(b[2], b[3])));
+      mt[c] = xhalf_max(xrow_max(mt[c])) * mul[c];
+      above |= ref[c].exceeded(mt[c], mt[c] + lv);
+    }
+    if (__any(above)) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const float ao = ref[c].raised(mt[c], mt[c] + lv);
 #pragma unroll
         for (int i = 0; i < VB; ++i) oacc[c][i] *= ao;
       }
-      const Q8Weight w = ref[c].weight(lv);
-      if (__any(w.lost)) {
+    }
+    Q8Weight w[NC];
+    bool lost = false;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      w[c] = ref[c].weight(lv);
+      lost |= w[c].lost;
+    }
+    if (__any(lost)) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
         float ps = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ps += fast_exp2(fmaf(e[i], mul, w.l_offset));
-        ref[c].l += w.lost ? ps : 0.f;
+        for (int i = 0; i < 8; ++i) ps += fast_exp2(fmaf(sacc[c][i >> 2][i & 3], mul[c], w[c].l_offset));
+        ref[c].l += w[c].lost ? ps : 0.f;
       }
-      float ps = 0.f;
+    }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        e[i] = fast_exp2(fmaf(e[i], mul, w.offset));
-        ps += e[i];
-      }
-      ref[c].l += ps * w.to_l;
+    for (int c = 0; c < NC; ++c) {
+      float e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = fast_exp2(fmaf(sacc[c][i >> 2][i & 3], mul[c], w[c].offset));
+      ref[c].l += (((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]))) * w[c].to_l;
 #pragma unroll
       for (int i = 0; i < 4; ++i) split2<TERMS>(e[2 * i], e[2 * i + 1], pk[c][i]);
     }
@@ -1208,10 +1229,11 @@ int q8_dpad(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 // Column blocks of 16 rows that a workgroup takes: as many as the registers of a lane
 // hold the sums of.  One block against two and four, each with its best split count:
 // 64 rows, D = 128, 8 x 100,000 keys of one KV head 129, 91 and 64 us; 64 rows, D = 64,
-// 64 x 8,000 keys 98, 66 and 40.  (With more, fp32 queries and D > 128 would spill.)
+// 64 x 8,000 keys 98, 66 and 40; 40 rows, D = 64, 16 x 8 heads x about 3,000 keys: 39 in
+// three blocks, 45 in four.  (With more, fp32 queries and D > 128 would spill.)
 static int q8_cols(int dtype, int D, int rows) {
   const int most = D > 128 ? 1 : dtype == SK_F32 ? 2 : 4;
-  const int want = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  const int want = rows <= 16 ? 1 : (rows + 15) / 16;
   return want < most ? want : most;
 }
 
@@ -1281,6 +1303,8 @@ static hipError_t launch_dp(const Q8AttnParams& p, hipStream_t s) {
   if (nc == 1) return launch_nc<C, TERMS, DP, 1>(p, s);
   if constexpr (DP <= 128)
     if (nc == 2) return launch_nc<C, TERMS, DP, 2>(p, s);
+  if constexpr (DP <= 128 && TERMS == 1)
+    if (nc == 3) return launch_nc<C, TERMS, DP, 3>(p, s);
   if constexpr (DP <= 128 && TERMS == 1)
     if (nc == 4) return launch_nc<C, TERMS, DP, 4>(p, s);
   return hipErrorInvalidValue;
