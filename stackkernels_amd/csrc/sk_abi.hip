@@ -1062,6 +1062,8 @@ static int check_q8(const sk_q8_shape* sh) {
     return fail(SK_EUNSUPPORTED, "head dim %d unsupported: need a multiple of 16 up to 256", D);
   if (block_size <= 0 || block_size % 32 != 0)
     return fail(SK_EINVAL, "block_size=%d must be a positive multiple of 32", block_size);
+  if (block_size > 1 << 24)  // (a block's elements are counted in 32 bits)
+    return fail(SK_EINVAL, "block_size=%d is more than 2^24", block_size);
   if (max_pages > 0) {
     if (rows <= 0 || rows % block_size != 0)
       return fail(SK_EINVAL, "page_size=%d must be a positive multiple of block_size=%d", rows,
@@ -1179,8 +1181,13 @@ int sk_kv_cache_update_q8(const sk_q8_shape* shape, const void* k, const void* v
       (rc = make_q8_cache("v_cache", v_cache, v_scale, sh.code_strides[1], sh.scale_strides[1], D,
                           paged, &p.c[1])))
     return rc;
-  for (int i = 0; i < 2; ++i)
-    if (rows > 1 && p.c[i].ss == 0) return fail(SK_EINVAL, "cache rows overlap (row stride 0)");
+  for (int i = 0; i < 2; ++i) {
+    const sk::Q8Cache& c = p.c[i];
+    if ((rows > 1 && c.ss == 0) || (Hkv > 1 && c.sh == 0) || (sh.units > 1 && c.sb == 0))
+      return fail(SK_EINVAL, "%s_cache rows overlap (stride 0)", i ? "v" : "k");
+    if ((rows > sh.block_size && c.cs == 0) || (Hkv > 1 && c.ch == 0) || (sh.units > 1 && c.cb == 0))
+      return fail(SK_EINVAL, "%s_scale entries overlap (stride 0)", i ? "v" : "k");
+  }
   if (rope_cos || rope_sin) {
     if ((rc = make_rope(rope_cos, rope_sin, rope_dtype, rope_rows, rope_stride, rope_pos,
                         rope_start, D, B > 0 ? T : 0, &p.rope)))
@@ -1273,7 +1280,7 @@ int sk_attn_q8(const sk_q8_shape* shape, const void* q, const void* k_cache, con
     return fail(SK_EWORKSPACE, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
   p.num_splits = num_splits;
   p.dpad = sk::q8_dpad(D);
-  const int per = sk::q8_rows_per_block(dtype, D, p.rows);
+  const int per = sk::q8_rows_per_block(dtype, p.rope.cos != nullptr, D, p.rows);
   p.row_blocks = (p.rows + per - 1) / per;
   if ((int64_t)B * Hkv * num_splits * p.row_blocks * 512 > 0xffffffffLL ||
       (num_splits > 1 && (int64_t)B * Hq * Sq * (num_splits > 16 ? 256 : 64) > 0xffffffffLL) ||

@@ -9,8 +9,8 @@
 // * q (rotated in fp32 where the call rotates) is divided by a power of two that
 //   brings its row's largest element into [1, 2), which its score's factor takes
 //   back: bf16 queries are then exact in fp16 (down to 2^-24 of the row's
-//   largest), rotated ones are rounded once to 11 bits.  fp32 queries are the sum
-//   of two such numbers (22 bits).
+//   largest), rotated ones are rounded once to 11 bits.  fp32 queries and rotated
+//   fp16 ones are the sum of two such numbers (22 bits).
 // * Probabilities e = 2^(s - m) are summed in fp32 into l and enter the product
 //   with V as fp16 numbers e t_n 2^(m - m2), where m2 is the running maximum of s
 //   + log2 t_n as m is that of s: largest contributions are near 1 whatever the
@@ -319,7 +319,8 @@ constexpr bool q8_q_in_lds() {
   return NC * DP > 256;
 }
 
-template <class C, int TERMS, int DP, int NC, int NW, bool PAGED>
+// QT, PT: fp16 terms of a query element, of a probability.
+template <class C, int QT, int PT, int DP, int NC, int NW, bool PAGED>
 __global__ void __launch_bounds__(NW * 64, 2) q8_attn_kernel(Q8AttnParams p) {
   constexpr int KC = DP / 64;   // 16-byte chunks of a K row per lane
   constexpr int KS = DP / 32;   // k-steps of S^T
@@ -328,7 +329,7 @@ __global__ void __launch_bounds__(NW * 64, 2) q8_attn_kernel(Q8AttnParams p) {
   constexpr bool kQLds = q8_q_in_lds<DP, NC>();
   // Where registers allow: V is taken from LDS before the softmax, and a score's
   // products run in two chains.
-  constexpr bool kEarly = NC * DP * TERMS <= 256;
+  constexpr bool kEarly = NC * DP * QT <= 256;
   constexpr int CH = NC == 1 ? 2 : 1;
 
   constexpr int ST = q8_stages<DP>();
@@ -341,7 +342,7 @@ __global__ void __launch_bounds__(NW * 64, 2) q8_attn_kernel(Q8AttnParams p) {
   __shared__ float red_l[NW][16 * NC];
   __shared__ __attribute__((aligned(1024))) uint8_t ring[RING > OUT ? RING : OUT];
   __shared__ float meta[NW][ST][4];  // of a stage: k's and v's scale, a page
-  __shared__ u32x4 qs[kQLds ? NC * KS * TERMS : 1][64];
+  __shared__ u32x4 qs[kQLds ? NC * KS * QT : 1][64];
   __shared__ float qmul_s[kQLds ? NC : 1][64];
 
   const int tid = threadIdx.x;
@@ -469,7 +470,7 @@ __global__ void __launch_bounds__(NW * 64, 2) q8_attn_kernel(Q8AttnParams p) {
 
   // Q^T operand: k-step s = 2 j + h of lane group g is head-dim columns 64 j +
   // 16 g + 8 h .. + 7, divided by 2^(exponent of the row's largest element).
-  u32x4 qreg[kQLds ? 1 : NC][KS][TERMS];
+  u32x4 qreg[kQLds ? 1 : NC][KS][QT];
   float qmul[NC];
   if (k_lo < k_hi) {
     auto col = [&](int s) SK_INLINE { return 64 * (s >> 1) + 16 * g + 8 * (s & 1); };
@@ -479,12 +480,12 @@ __global__ void __launch_bounds__(NW * 64, 2) q8_attn_kernel(Q8AttnParams p) {
       const int r = row0 + 16 * c + c16;
       if constexpr (kQLds) {
         if (c % NW != wave) continue;
-        qmul_s[c][lane] = q8_query<KS, TERMS>(p, b, hkv, r, sp.ql, col, reduce, qreg[0]);
+        qmul_s[c][lane] = q8_query<KS, QT>(p, b, hkv, r, sp.ql, col, reduce, qreg[0]);
 #pragma unroll
-        for (int i = 0; i < KS * TERMS; ++i)
-          qs[c * KS * TERMS + i][lane] = qreg[0][i / TERMS][i % TERMS];
+        for (int i = 0; i < KS * QT; ++i)
+          qs[c * KS * QT + i][lane] = qreg[0][i / QT][i % QT];
       } else {
-        qmul[c] = q8_query<KS, TERMS>(p, b, hkv, r, sp.ql, col, reduce, qreg[c]);
+        qmul[c] = q8_query<KS, QT>(p, b, hkv, r, sp.ql, col, reduce, qreg[c]);
       }
     }
     if constexpr (kQLds) {
@@ -538,10 +539,10 @@ __global__ void __launch_bounds__(NW * 64, 2) q8_attn_kernel(Q8AttnParams p) {
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int u = TERMS - 1; u >= 0; --u) {
+          for (int u = QT - 1; u >= 0; --u) {
             u32x4 q;
             if constexpr (kQLds)
-              q = qs[(c * KS + 2 * j + h) * TERMS + u][lane];
+              q = qs[(c * KS + 2 * j + h) * QT + u][lane];
             else
               q = qreg[c][2 * j + h][u];
 #pragma unroll
@@ -581,7 +582,7 @@ __global__ void __launch_bounds__(NW * 64, 2) q8_attn_kernel(Q8AttnParams p) {
 
     const bool masked = !ok || n0 + 32 > k_hi || n0 + 32 > sp.full;
     const float lv = __builtin_amdgcn_logf(vs);  // log2
-    uint32_t pk[NC][4][TERMS];
+    uint32_t pk[NC][4][PT];
     // All blocks' maxima first and one test for all of them: their chains then run
     // side by side.
     float mul[NC], mt[NC];
@@ -631,7 +632,7 @@ __global__ void __launch_bounds__(NW * 64, 2) q8_attn_kernel(Q8AttnParams p) {
       for (int i = 0; i < 8; ++i) e[i] = fast_exp2(fmaf(sacc[c][i >> 2][i & 3], mul[c], w[c].offset));
       ref[c].l += (((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]))) * w[c].to_l;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) split2<TERMS>(e[2 * i], e[2 * i + 1], pk[c][i]);
+      for (int i = 0; i < 4; ++i) split2<PT>(e[2 * i], e[2 * i + 1], pk[c][i]);
     }
     if constexpr (!kEarly) read_v();
     auto product = [&](int w, auto hc) SK_INLINE {
@@ -647,7 +648,7 @@ __global__ void __launch_bounds__(NW * 64, 2) q8_attn_kernel(Q8AttnParams p) {
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int u = TERMS - 1; u >= 0; --u) {
+        for (int u = PT - 1; u >= 0; --u) {
           const u32x4 pb = {pk[c][0][u], pk[c][1][u], pk[c][2][u], pk[c][3][u]};
           oacc[c][blk] = mfma16<F16>(a0, pb, oacc[c][blk]);
           oacc[c][blk + 1] = mfma16<F16>(a1, pb, oacc[c][blk + 1]);
@@ -760,7 +761,7 @@ constexpr int kQ8BigWaves = 8;
 constexpr int kQ8BigRows = 32 * kQ8BigWaves;
 
 // PARTS: pages a tile may lie in (1: contiguous caches, pages of whole tiles).
-template <class C, int DP, bool PAGED, int PARTS>
+template <class C, int QT, int DP, bool PAGED, int PARTS>
 __global__ void __launch_bounds__(kQ8BigWaves * 64) q8_big_kernel(Q8AttnParams p) {
   using L = Q8Big<DP>;
   constexpr int NT = kQ8BigWaves * 64;
@@ -890,7 +891,7 @@ __global__ void __launch_bounds__(kQ8BigWaves * 64) q8_big_kernel(Q8AttnParams p
     }
   };
 
-  u32x4 q[KS][1];
+  u32x4 q[KS][QT];
   f32x16 oacc[DB];
 #pragma unroll
   for (int i = 0; i < DB; ++i) oacc[i] = f32x16{};
@@ -990,7 +991,10 @@ __global__ void __launch_bounds__(kQ8BigWaves * 64) q8_big_kernel(Q8AttnParams p
       if constexpr (kNow && i + OLEAD >= NS && i + OLEAD - NS < NO)
         vt[i + OLEAD - NS] = read_v(i + OLEAD - NS);
       if constexpr (i < NS) {
-        if constexpr (kNext) nx = mfma32<F16>(a[i], q[i][0], nx);
+        if constexpr (kNext) {
+#pragma unroll
+          for (int k = QT - 1; k >= 0; --k) nx = mfma32<F16>(a[i], q[i][k], nx);
+        }
       } else if constexpr (kNow) {
         constexpr int j = i - NS;
         oacc[j % DB] = mfma32<F16>(vt[j], pk[j / DB], oacc[j % DB]);
@@ -1046,7 +1050,7 @@ __global__ void __launch_bounds__(kQ8BigWaves * 64) q8_big_kernel(Q8AttnParams p
     load_v(0, pg0);
     const float sv0 = load_scale(0, pg0);
     float sv = load_scale(1, pg1);
-    qmul = q8_query<KS, 1>(
+    qmul = q8_query<KS, QT>(
         p, b, hkv, r, sp.ql, [&](int s) SK_INLINE { return 16 * s + 8 * hi2; },
         [](float x) SK_INLINE { return xhalf_max(x); }, q);
     static_for<8>([&](auto st) SK_INLINE { widen_k(0, st); });
@@ -1061,7 +1065,11 @@ __global__ void __launch_bounds__(kQ8BigWaves * 64) q8_big_kernel(Q8AttnParams p
     settle_scales(sv0, pg0);
     if (w_tiles > 0) {
 #pragma unroll
-      for (int s = 0; s < KS; ++s) sa = mfma32<F16>(lds_read_b128(kfrom + 16 * s), q[s][0], sa);
+      for (int s = 0; s < KS; ++s) {
+        const u32x4 a = lds_read_b128(kfrom + 16 * s);
+#pragma unroll
+        for (int k = QT - 1; k >= 0; --k) sa = mfma32<F16>(a, q[s][k], sa);
+      }
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sa[i]);
       settle(k_lo, std::integral_constant<int, 0>{}, sa, mx);
@@ -1226,13 +1234,20 @@ static hipError_t launch_combine(const Q8AttnParams& p, hipStream_t s) {
 
 int q8_dpad(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
+// Whether a query element takes two fp16 terms: fp32 queries, and fp16 ones that are
+// rotated (which one term would round a second time, to the precision of the result:
+// twice its error over long rows).  bf16 results are coarser than one term.
+static bool q8_two_terms(int dtype, bool rotated) {
+  return dtype == SK_F32 || (dtype == SK_F16 && rotated);
+}
+
 // Column blocks of 16 rows that a workgroup takes: as many as the registers of a lane
 // hold the sums of.  One block against two and four, each with its best split count:
 // 64 rows, D = 128, 8 x 100,000 keys of one KV head 129, 91 and 64 us; 64 rows, D = 64,
 // 64 x 8,000 keys 98, 66 and 40; 40 rows, D = 64, 16 x 8 heads x about 3,000 keys: 39 in
 // three blocks, 45 in four.  (With more, fp32 queries and D > 128 would spill.)
-static int q8_cols(int dtype, int D, int rows) {
-  const int most = D > 128 ? 1 : dtype == SK_F32 ? 2 : 4;
+static int q8_cols(int dtype, bool rotated, int D, int rows) {
+  const int most = D > 128 ? 1 : dtype == SK_F32 ? 2 : D > 64 && q8_two_terms(dtype, rotated) ? 3 : 4;
   const int want = rows <= 16 ? 1 : (rows + 15) / 16;
   return want < most ? want : most;
 }
@@ -1245,12 +1260,12 @@ static bool q8_big(int dtype, int D, int rows) {
   return dtype != SK_F32 && D <= 128 && rows > 64;
 }
 
-int q8_rows_per_block(int dtype, int D, int rows) {
-  return q8_big(dtype, D, rows) ? kQ8BigRows : 16 * q8_cols(dtype, D, rows);
+int q8_rows_per_block(int dtype, bool rotated, int D, int rows) {
+  return q8_big(dtype, D, rows) ? kQ8BigRows : 16 * q8_cols(dtype, rotated, D, rows);
 }
 
 int q8_splits(int dtype, int B, int Hkv, int rows, int keys, int D) {
-  const int per = q8_rows_per_block(dtype, D, rows);
+  const int per = q8_rows_per_block(dtype, false, D, rows);
   const int64_t units = (int64_t)B * Hkv * ((rows + per - 1) / per);
   if (units <= 0) return 1;
   if (q8_big(dtype, D, rows)) {
@@ -1286,54 +1301,54 @@ int q8_splits(int dtype, int B, int Hkv, int rows, int keys, int D) {
   return best;
 }
 
-template <class C, int TERMS, int DP, int NC>
+template <class C, int QT, int PT, int DP, int NC>
 static hipError_t launch_nc(const Q8AttnParams& p, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)p.B * p.Hkv * p.num_splits * p.row_blocks));
   constexpr int NW = q8_waves<DP, NC>();
   if (p.table)
-    hipLaunchKernelGGL((q8_attn_kernel<C, TERMS, DP, NC, NW, true>), grid, dim3(NW * 64), 0, s, p);
+    hipLaunchKernelGGL((q8_attn_kernel<C, QT, PT, DP, NC, NW, true>), grid, dim3(NW * 64), 0, s, p);
   else
-    hipLaunchKernelGGL((q8_attn_kernel<C, TERMS, DP, NC, NW, false>), grid, dim3(NW * 64), 0, s, p);
+    hipLaunchKernelGGL((q8_attn_kernel<C, QT, PT, DP, NC, NW, false>), grid, dim3(NW * 64), 0, s, p);
   return hipGetLastError();
 }
 
-template <class C, int TERMS, int DP>
+template <class C, int QT, int PT, int DP>
 static hipError_t launch_dp(const Q8AttnParams& p, hipStream_t s) {
-  const int nc = q8_cols(p.dtype, p.D, p.rows);
-  if (nc == 1) return launch_nc<C, TERMS, DP, 1>(p, s);
+  const int nc = q8_cols(p.dtype, p.rope.cos != nullptr, p.D, p.rows);
+  if (nc == 1) return launch_nc<C, QT, PT, DP, 1>(p, s);
   if constexpr (DP <= 128)
-    if (nc == 2) return launch_nc<C, TERMS, DP, 2>(p, s);
-  if constexpr (DP <= 128 && TERMS == 1)
-    if (nc == 3) return launch_nc<C, TERMS, DP, 3>(p, s);
-  if constexpr (DP <= 128 && TERMS == 1)
-    if (nc == 4) return launch_nc<C, TERMS, DP, 4>(p, s);
+    if (nc == 2) return launch_nc<C, QT, PT, DP, 2>(p, s);
+  if constexpr (DP <= 128 && PT == 1)
+    if (nc == 3) return launch_nc<C, QT, PT, DP, 3>(p, s);
+  if constexpr (PT == 1 && (DP == 64 || (DP == 128 && QT == 1)))
+    if (nc == 4) return launch_nc<C, QT, PT, DP, 4>(p, s);
   return hipErrorInvalidValue;
 }
 
-template <class C, int DP>
+template <class C, int QT, int DP>
 static hipError_t launch_big(const Q8AttnParams& p, hipStream_t s) {
   using L = Q8Big<DP>;
   const dim3 block(kQ8BigWaves * 64);
   const dim3 grid((unsigned)((int64_t)p.B * p.Hkv * p.num_splits * p.row_blocks));
   if (!p.table) {
-    hipLaunchKernelGGL((q8_big_kernel<C, DP, false, 1>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((q8_big_kernel<C, QT, DP, false, 1>), grid, block, 0, s, p);
     return hipGetLastError();
   }
   if (p.page_size % L::BN != 0)
-    hipLaunchKernelGGL((q8_big_kernel<C, DP, true, L::NH>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((q8_big_kernel<C, QT, DP, true, L::NH>), grid, block, 0, s, p);
   else
-    hipLaunchKernelGGL((q8_big_kernel<C, DP, true, 1>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((q8_big_kernel<C, QT, DP, true, 1>), grid, block, 0, s, p);
   return hipGetLastError();
 }
 
-template <class C, int TERMS>
+template <class C, int QT, int PT>
 static hipError_t launch_ct(const Q8AttnParams& p, hipStream_t s) {
-  if (q8_big(p.dtype, p.D, p.rows)) {
-    return p.D <= 64 ? launch_big<C, 64>(p, s) : launch_big<C, 128>(p, s);
-  }
-  if (p.D <= 64) return launch_dp<C, TERMS, 64>(p, s);
-  if (p.D <= 128) return launch_dp<C, TERMS, 128>(p, s);
-  return launch_dp<C, TERMS, 256>(p, s);
+  if constexpr (PT == 1)
+    if (q8_big(p.dtype, p.D, p.rows))
+      return p.D <= 64 ? launch_big<C, QT, 64>(p, s) : launch_big<C, QT, 128>(p, s);
+  if (p.D <= 64) return launch_dp<C, QT, PT, 64>(p, s);
+  if (p.D <= 128) return launch_dp<C, QT, PT, 128>(p, s);
+  return launch_dp<C, QT, PT, 256>(p, s);
 }
 
 hipError_t launch_q8_attn(int code, const Q8AttnParams& p0, hipStream_t s) {
@@ -1343,10 +1358,12 @@ hipError_t launch_q8_attn(int code, const Q8AttnParams& p0, hipStream_t s) {
   p.hkv_div = FastDiv(p.Hkv);
   p.split_div = FastDiv(p.num_splits);
   p.block_rows_div = FastDiv(p.row_blocks);
-  const bool wide = p.dtype == SK_F32;
-  const hipError_t e =
-      code == kCodeI8 ? (wide ? launch_ct<I8, 2>(p, s) : launch_ct<I8, 1>(p, s))
-                      : (wide ? launch_ct<E4M3, 2>(p, s) : launch_ct<E4M3, 1>(p, s));
+  const bool two = q8_two_terms(p.dtype, p.rope.cos != nullptr);
+  auto launch = [&](auto c) {
+    using C = decltype(c);
+    return p.dtype == SK_F32 ? launch_ct<C, 2, 2>(p, s) : two ? launch_ct<C, 2, 1>(p, s) : launch_ct<C, 1, 1>(p, s);
+  };
+  const hipError_t e = code == kCodeI8 ? launch(I8{}) : launch(E4M3{});
   if (e != hipSuccess || p.num_splits == 1) return e;
   return p.dpad == 64 ? launch_combine<64>(p, s) : p.dpad == 128 ? launch_combine<128>(p, s) : launch_combine<256>(p, s);
 }

@@ -329,7 +329,7 @@ def flash_attention_q8(
         k, v: codes, ``int8`` or ``float8_e4m3fn``, (B, H_kv, S_k, D) or page pools
             (num_pages, H_kv, page_size, D); 16-byte-aligned rows, contiguous D.
         k_scale, v_scale: float32 (B, H_kv, ceil(S_k / block_size)) or (num_pages,
-            H_kv, page_size / block_size).
+            H_kv, page_size / block_size), finite and not negative.
         is_causal: query i of a row with n keys and m queries sees keys ``j <= n - m
             + i`` (bottom-right aligned); else all n.
         sm_scale: score scale, default 1/sqrt(D).
@@ -561,9 +561,75 @@ def _register_decode_ops() -> None:
     _LIBS.append(lib)
 
 
+def _register_q8_ops() -> None:
+    """``torch.ops.stackkernels_amd.attention_q8`` and ``kv_cache_update_q8``: the
+    calls over an 8-bit cache for compiled graphs, with every argument, as
+    ``decode`` is for ``flash_decode``."""
+
+    @torch.library.custom_op("stackkernels_amd::attention_q8", mutates_args=())
+    def _attention_q8_op(
+        q: torch.Tensor,
+        k: torch.Tensor,
+        v: torch.Tensor,
+        k_scale: torch.Tensor,
+        v_scale: torch.Tensor,
+        is_causal: bool,
+        sm_scale: float,
+        cache_seqlens: torch.Tensor | None,
+        block_table: torch.Tensor | None,
+        query_lens: torch.Tensor | None,
+        block_size: int,
+        rope_cos: torch.Tensor | None,
+        rope_sin: torch.Tensor | None,
+        rope_positions: torch.Tensor | None,
+        start_pos: int,
+    ) -> torch.Tensor:
+        pos = rope_positions if rope_positions is not None else start_pos
+        return flash_attention_q8(q, k, v, k_scale, v_scale, is_causal, sm_scale, cache_seqlens,
+                                  block_table, query_lens, block_size=block_size,
+                                  rope_cos=rope_cos, rope_sin=rope_sin, start_pos=pos)
+
+    @_attention_q8_op.register_fake
+    def _attention_q8_fake(q, k, v, k_scale, v_scale, is_causal, sm_scale, cache_seqlens,
+                           block_table, query_lens, block_size, rope_cos, rope_sin,
+                           rope_positions, start_pos):
+        return q.new_empty(q.shape)
+
+    @torch.library.custom_op("stackkernels_amd::kv_cache_update_q8",
+                             mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"))
+    def _update_q8_op(
+        k: torch.Tensor,
+        v: torch.Tensor,
+        k_cache: torch.Tensor,
+        v_cache: torch.Tensor,
+        k_scale: torch.Tensor,
+        v_scale: torch.Tensor,
+        cache_seqlens: torch.Tensor,
+        new_lens: torch.Tensor | None,
+        block_table: torch.Tensor | None,
+        block_size: int,
+        rope_cos: torch.Tensor | None,
+        rope_sin: torch.Tensor | None,
+        rope_positions: torch.Tensor | None,
+        start_pos: int,
+    ) -> None:
+        from stackkernels_amd.torch.cache import kv_cache_update_q8
+
+        pos = rope_positions if rope_positions is not None else start_pos
+        kv_cache_update_q8(k, v, k_cache, v_cache, k_scale, v_scale, cache_seqlens, new_lens,
+                           block_table, block_size=block_size, rope_cos=rope_cos,
+                           rope_sin=rope_sin, start_pos=pos)
+
+    @_update_q8_op.register_fake
+    def _update_q8_fake(k, v, k_cache, v_cache, k_scale, v_scale, cache_seqlens, new_lens,
+                        block_table, block_size, rope_cos, rope_sin, rope_positions, start_pos):
+        return None
+
+
 _LIBS: list = []
 _CUSTOM_OP_REGISTERED = _register_ops()
 _register_decode_ops()
+_register_q8_ops()
 
 
 __all__ = [
