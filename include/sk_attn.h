@@ -590,7 +590,7 @@ SK_API int sk_attn_q8_plan(int dtype, int B, int Hq, int Hkv, int Sq, int Sk, in
 
 /*
  * Attention of Sq >= 1 query tokens per batch row over a cache of 8-bit codes
- * (the format of sk_kv_cache_update_q8; scales may be any fp32 numbers).
+ * (the format of sk_kv_cache_update_q8; scales finite and not negative).
  *
  *   q (B, Hq, Sq, D) -> o (B, Hq, Sq, D) of q's dtype.
  *

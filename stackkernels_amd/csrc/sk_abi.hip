@@ -1280,7 +1280,7 @@ int sk_attn_q8(const sk_q8_shape* shape, const void* q, const void* k_cache, con
     return fail(SK_EWORKSPACE, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
   p.num_splits = num_splits;
   p.dpad = sk::q8_dpad(D);
-  const int per = sk::q8_rows_per_block(dtype, p.rope.cos != nullptr, D, p.rows);
+  const int per = sk::q8_rows_per_block(dtype, D, p.rows);
   p.row_blocks = (p.rows + per - 1) / per;
   if ((int64_t)B * Hkv * num_splits * p.row_blocks * 512 > 0xffffffffLL ||
       (num_splits > 1 && (int64_t)B * Hq * Sq * (num_splits > 16 ? 256 : 64) > 0xffffffffLL) ||

@@ -22,9 +22,9 @@
 // Layout.  S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16 with 16 (query
 // token, head) rows of one KV head as the 16 columns, NC such blocks per wave.  A
 // wave takes 32 keys at a time through LDS of its own, which loads fill that pass no
-// register: up to two tiles are on their way while one is worked on, and no wave waits
-// for another before the end.  (Loads into registers instead: 655 -> 804 us for 64 x
-// 32,000 keys, D = 128, where the second wave of a SIMD did not fit.)
+// register: the next tile is on its way while one is worked on, and no wave waits for
+// another before the end.  (Loads into registers instead: 804 us for 655 at 64 x 8 heads
+// x 32,768 keys, D = 128, where the second wave of a SIMD did not fit.)
 // * Row 4 a + b of a 16-row operand block of K is key 4 b + a, so that group g's four
 //   results are keys 4 b + g and each load of V below covers whole rows.
 // * K: lane (key r, group g) brings the 16 bytes 64 j + 16 g of its key's row and
@@ -35,8 +35,8 @@
 //   the columns VB m + c, so the transposition V^T needs is a byte selection.
 // The waves of a workgroup take tiles in turn and merge their sums in LDS.
 //
-// What bounds it: long caches of many rows HBM (64 x 8 KV heads x 32,000 keys, D = 128:
-// 4.3 GB of codes in 655 us, 6.6 TB/s); few or short ones the chain of one tile, loads,
+// What bounds it: long caches of many rows HBM (64 x 8 KV heads x 32,768 keys, D = 128:
+// 4.3 GB of codes in 673 us, 6.4 TB/s); few or short ones the chain of one tile, loads,
 // scores, maximum, probabilities, sums, about 1 us an iteration at D = 128.
 #include <type_traits>
 #include <utility>
@@ -304,11 +304,14 @@ template <int DP, int NC>
 constexpr int q8_waves() {
   return NC * DP > 256 ? 8 : 4;
 }
-// Tiles in flight per wave: two, one where they take 16 KB each (two would leave a CU
-// four waves).
+// Tiles in flight per wave: two of 4 KB, one of 8 KB or more, where a CU's other
+// workgroups keep it loading.  (Two of 8 KB: 64 query heads of one KV head, 8 x 100,000
+// keys 65 us for 60; 300 x 8 heads x 300 keys 57 for 42; 32 x 8 heads, up to 4,096 keys
+// each, 43 for 41; only 64 x 8 heads x 32,768 keys gain, 655 for 673.  One of 4 KB: 16 x
+// 8 heads x 3,000 keys, 40 rows 43 us for 38.)
 template <int DP>
 constexpr int q8_stages() {
-  return DP > 128 ? 1 : 2;
+  return DP > 64 ? 1 : 2;
 }
 
 // Column blocks whose queries are read from LDS each tile (the waves share them): with
@@ -1246,8 +1249,8 @@ static bool q8_two_terms(int dtype, bool rotated) {
 // 64 rows, D = 128, 8 x 100,000 keys of one KV head 129, 91 and 64 us; 64 rows, D = 64,
 // 64 x 8,000 keys 98, 66 and 40; 40 rows, D = 64, 16 x 8 heads x about 3,000 keys: 39 in
 // three blocks, 45 in four.  (With more, fp32 queries and D > 128 would spill.)
-static int q8_cols(int dtype, bool rotated, int D, int rows) {
-  const int most = D > 128 ? 1 : dtype == SK_F32 ? 2 : D > 64 && q8_two_terms(dtype, rotated) ? 3 : 4;
+static int q8_cols(int dtype, int D, int rows) {
+  const int most = D > 128 ? 1 : dtype == SK_F32 ? 2 : 4;
   const int want = rows <= 16 ? 1 : (rows + 15) / 16;
   return want < most ? want : most;
 }
@@ -1260,12 +1263,12 @@ static bool q8_big(int dtype, int D, int rows) {
   return dtype != SK_F32 && D <= 128 && rows > 64;
 }
 
-int q8_rows_per_block(int dtype, bool rotated, int D, int rows) {
-  return q8_big(dtype, D, rows) ? kQ8BigRows : 16 * q8_cols(dtype, rotated, D, rows);
+int q8_rows_per_block(int dtype, int D, int rows) {
+  return q8_big(dtype, D, rows) ? kQ8BigRows : 16 * q8_cols(dtype, D, rows);
 }
 
 int q8_splits(int dtype, int B, int Hkv, int rows, int keys, int D) {
-  const int per = q8_rows_per_block(dtype, false, D, rows);
+  const int per = q8_rows_per_block(dtype, D, rows);
   const int64_t units = (int64_t)B * Hkv * ((rows + per - 1) / per);
   if (units <= 0) return 1;
   if (q8_big(dtype, D, rows)) {
@@ -1281,20 +1284,22 @@ int q8_splits(int dtype, int B, int Hkv, int rows, int keys, int D) {
     }
     return best;
   }
-  // Microseconds, from times of 34 shapes over 1 to 128 splits (the chosen count came
-  // within 10% of the best one's time in all of them): a CU gets through an iteration
-  // (32 keys a wave) of its workgroups in about `step` however many it holds (at D <= 64
-  // three quarters of it past the first); 1.5 + nc is a workgroup's own cost; a quarter of its time is lost at the end, where CUs finish
+  // Microseconds, from times of 40 shapes over 1 to 128 splits: a workgroup's iteration
+  // (32 keys a wave) takes `step`; a CU gets through its workgroups one after the other,
+  // or in three quarters of that where registers and LDS let it hold two or more; 1.5 + nc is a
+  // workgroup's own cost; a quarter of its time is lost at the end, where CUs finish
   // unevenly; splits cost the second kernel and the partials' traffic.
   const int nc = per / 16, dp = q8_dpad(D), waves = nc * dp > 256 ? 8 : 4;
-  const double step = (0.4 + 0.36 * dp / 64) * (1 + 0.3 * (nc - 1)) * (waves == 8 ? 1.4 : 1.0);
+  const bool shares = dp == 64 || (dp == 128 && nc <= 2);
+  const double step = (dp == 64 ? 0.76 : dp == 256 ? 1.84 : nc == 1 ? 1.3 : 1.12) *
+                      (1 + 0.3 * (nc - 1)) * (waves == 8 ? 1.4 : 1.0);
   const int tiles = (keys + 31) / 32;
   int best = 1;
   double least = 1e30;
-  for (int s = 1; s <= kQ8MaxSplits && (s == 1 || s <= tiles / 2); ++s) {
+  for (int s = 1; s <= 128 && (s == 1 || s <= tiles / 2); ++s) {
     const double run = ((tiles + s - 1) / s + waves - 1) / waves * step;
     const double held = (double)((units * s + 255) / 256);
-    const double cost = (dp > 64 ? held : 0.25 + 0.75 * held) * (run + 1.5 + nc) + 0.25 * run +
+    const double cost = (shares ? 0.25 + 0.75 * held : held) * (run + 1.5 + nc) + 0.25 * run +
                         (s > 1 ? 3 + (double)B * Hkv * rows * s * dp * 2.5e-6 : 0);
     if (cost < 0.99 * least) least = cost, best = s;
   }
@@ -1314,13 +1319,13 @@ static hipError_t launch_nc(const Q8AttnParams& p, hipStream_t s) {
 
 template <class C, int QT, int PT, int DP>
 static hipError_t launch_dp(const Q8AttnParams& p, hipStream_t s) {
-  const int nc = q8_cols(p.dtype, p.rope.cos != nullptr, p.D, p.rows);
+  const int nc = q8_cols(p.dtype, p.D, p.rows);
   if (nc == 1) return launch_nc<C, QT, PT, DP, 1>(p, s);
   if constexpr (DP <= 128)
     if (nc == 2) return launch_nc<C, QT, PT, DP, 2>(p, s);
   if constexpr (DP <= 128 && PT == 1)
     if (nc == 3) return launch_nc<C, QT, PT, DP, 3>(p, s);
-  if constexpr (PT == 1 && (DP == 64 || (DP == 128 && QT == 1)))
+  if constexpr (DP <= 128 && PT == 1)
     if (nc == 4) return launch_nc<C, QT, PT, DP, 4>(p, s);
   return hipErrorInvalidValue;
 }

@@ -109,7 +109,7 @@ hipError_t launch_q8_append(int dtype, int code, const Q8AppendParams& p, hipStr
 hipError_t launch_q8_attn(int code, const Q8AttnParams& p, hipStream_t s);
 // Rows of a KV head (query tokens x group) that one workgroup takes, and the
 // split count for a shape (keys: the most keys a row can see).
-int q8_rows_per_block(int dtype, bool rotated, int D, int rows);
+int q8_rows_per_block(int dtype, int D, int rows);
 int q8_splits(int dtype, int B, int Hkv, int rows, int keys, int D);
 int q8_dpad(int D);
 
