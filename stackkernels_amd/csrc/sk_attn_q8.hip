@@ -1274,7 +1274,7 @@ int q8_splits(int dtype, int B, int Hkv, int rows, int keys, int D) {
   if (q8_big(dtype, D, rows)) {
     // Rounds of the 256 CUs (one workgroup each) times a piece's tiles and the fixed
     // cost of a workgroup and of a row's partials, in tiles.
-    const int tiles = (keys * (D <= 64 ? 64 : 128) + 8191) / 8192;
+    const int tiles = (int)(((int64_t)keys * (D <= 64 ? 64 : 128) + 8191) / 8192);
     int best = 1;
     double least = 1e30;
     for (int s = 1; s <= 64 && (s == 1 || 2 * s <= tiles); ++s) {
@@ -1286,9 +1286,10 @@ int q8_splits(int dtype, int B, int Hkv, int rows, int keys, int D) {
   }
   // Microseconds, from times of 40 shapes over 1 to 128 splits: a workgroup's iteration
   // (32 keys a wave) takes `step`; a CU gets through its workgroups one after the other,
-  // or in three quarters of that where registers and LDS let it hold two or more; 1.5 + nc is a
-  // workgroup's own cost; a quarter of its time is lost at the end, where CUs finish
-  // unevenly; splits cost the second kernel and the partials' traffic.
+  // or in three quarters of that where registers and LDS let it hold several; 1.5 + nc is
+  // a workgroup's own cost; a quarter of its time is lost at the end, where CUs finish
+  // unevenly; splits cost the second kernel and the partials' traffic.  The count it
+  // takes came within 10% of the best one's time.
   const int nc = per / 16, dp = q8_dpad(D), waves = nc * dp > 256 ? 8 : 4;
   const bool shares = dp == 64 || (dp == 128 && nc <= 2);
   const double step = (dp == 64 ? 0.76 : dp == 256 ? 1.84 : nc == 1 ? 1.3 : 1.12) *

@@ -144,6 +144,17 @@ def test_plan_of_empty_shapes(lib):
         assert ns.value == 1 and nb.value == 0
 
 
+def test_plan_of_the_longest_caches(lib):
+    """A hundred million keys and 2^31 - 2^16 of them: no count overflows, and one row's
+    many keys are shared out."""
+    for dtype, sq in ((2, 1), (2, 100), (0, 1), (1, 40)):
+        for sk in (100_000_000, 0x7fff0000):
+            ns, nb = ctypes.c_int(-1), ctypes.c_size_t(0)
+            assert lib.sk_attn_q8_plan(dtype, 1, 8, 1, sq, sk, 128, 1, ctypes.byref(ns),
+                                       ctypes.byref(nb)) == 0
+            assert 16 <= ns.value <= 256
+
+
 @pytest.mark.parametrize("dtype", [0, 1, 2])
 @pytest.mark.parametrize("d", [16, 64, 128, 256])
 def test_plan_splits_fit(lib, dtype, d):
