@@ -87,19 +87,19 @@ PEAK_NOTE = {
 # so these are recorded figures.  TRAFFIC_SOURCES_SHA256 is the digest of the
 # kernel sources (kernel_sources_digest) the counters were measured on; when
 # the sources differ, the line reports traffic null rather than a stale figure.
-TRAFFIC_SOURCES_SHA256 = "caf67ddc427234fcfa34719631437866058f68af6a620cbe94e3947be4e70ea7"
+TRAFFIC_SOURCES_SHA256 = "40678798a0a4b05958d2e9c9d8acb50dd3df5e40826c8e53b81073361c3ae2a5"
 HBM_TRAFFIC_BYTES = {
-    "fwd": 680_866_517,
-    "fwd_long": 844_129_003,
-    "fwdbwd": 4_537_413_755,
-    "decode": 8_601_609_571,
-    "decode_mqa": 573_052_245,
-    "decode_varlen": 4_305_237_180,
-    "kv_update": 67_240_132,
-    "decode_paged": 4_305_384_459,
-    "decode_rope": 8_601_623_879,
-    "kv_update_rope": 75_523_343,
-    "decode_step": 4_306_766_909,
+    "fwd": 681_152_708,
+    "fwd_long": 843_776_871,
+    "fwdbwd": 4_537_064_167,
+    "decode": 8_601_609_486,
+    "decode_mqa": 573_052_340,
+    "decode_varlen": 4_305_237_104,
+    "kv_update": 67_240_131,
+    "decode_paged": 4_305_384_394,
+    "decode_rope": 8_601_623_863,
+    "kv_update_rope": 75_523_338,
+    "decode_step": 4_306_767_132,
 }
 
 
