@@ -192,6 +192,16 @@ def test_page_plan_argument_errors(lib):
     assert plan(B=0) == _lib.SK_OK
 
 
+def test_build_refuses_spills():
+    """The kernel of few rows counts its loads: a build that spills is refused."""
+    from stackkernels_amd.csrc import build
+
+    text = "Function Name: _ZN2sk14q8_attn_kernelI\n ScratchSize [bytes/lane]: %d"
+    build._check_no_scratch("sk_attn_q8.hip", text % 0)
+    with pytest.raises(RuntimeError, match="spills 8 bytes"):
+        build._check_no_scratch("sk_attn_q8.hip", text % 8)
+
+
 def _inputs(code, seed=0):
     kc, ks = _q8.make_cache(2, 2, 96, 32, 32, code, seed)
     vc, vs = _q8.make_cache(2, 2, 96, 32, 32, code, seed + 1)
