@@ -1257,8 +1257,9 @@ static int q8_cols(int dtype, int D, int rows) {
 
 // Whether the kernel of many rows runs (16-bit queries): from 65 rows of a KV head
 // on.  8 KV heads of D = 128, each with its best split count, first kernel and this
-// one: 16 x 8,000 keys 64 and 93 us at 32 rows, 96 and 110 at 64, 144 and 123 at 96,
-// 291 and 186 at 256; 1 x 16,000 keys 25 and 27, 29 and 29, 35 and 31, 50 and 42.
+// one: 16 x 8,000 keys 61 and 94 us at 32 rows, 81 and 110 at 64, 117 and 118 at 96, 121
+// and 131 at 128, 222 and 187 at 256; 1 x 16,000 keys 20 and 23, 28 and 24, 30 and 27,
+// 31 and 29, 42 and 41.
 static bool q8_big(int dtype, int D, int rows) {
   return dtype != SK_F32 && D <= 128 && rows > 64;
 }
